@@ -51,6 +51,44 @@ class pt_backward_buf_t(C.Structure):
                  "d_hid2_all", "drt_ffn_all")]
 
 
+# Serving operators (include/ptc_serve.h). Pointers are device addresses.
+PTC_F32, PTC_F16, PTC_BF16 = 0, 1, 2
+PTC_SERVE_ERR_PAGES, PTC_SERVE_ERR_TABLE, PTC_SERVE_ERR_TOKENS = 1, 2, 4
+PTC_SERVE_ERR_LENGTH, PTC_SERVE_ERR_INDEX = 8, 16
+PTC_ATTN_WORKSPACE_BYTES = 64 << 20
+
+
+class ptc_pages_args(C.Structure):
+    _fields_ = ([(n, C.c_int) for n in ("n_seqs", "page_size", "max_pages", "max_tokens", "n_free", "n_pages")]
+                + [(n, vp) for n in ("past_len", "new_len", "free_pages", "page_table", "kv_len", "q_start", "slots",
+                                     "positions", "pages_used", "err")])
+
+
+class ptc_paged_cache(C.Structure):
+    _fields_ = ([("k", vp), ("v", vp)]
+                + [(n, C.c_int) for n in ("dtype", "n_pages", "page_size", "n_kv_heads", "head_dim")]
+                + [(n, C.c_longlong) for n in ("page_stride", "head_stride", "token_stride")])
+
+
+class ptc_append_args(C.Structure):
+    _fields_ = [("cache", ptc_paged_cache), ("n_tokens", C.c_int), ("n_heads", C.c_int), ("q", vp), ("k", vp), ("v", vp),
+                ("q_stride", C.c_longlong), ("k_stride", C.c_longlong), ("v_stride", C.c_longlong),
+                ("positions", vp), ("slots", vp), ("rope", vp), ("n_pos", C.c_int), ("q_out", vp),
+                ("q_out_stride", C.c_longlong), ("err", vp)]
+
+
+class ptc_attn_args(C.Structure):
+    _fields_ = [("cache", ptc_paged_cache), ("n_seqs", C.c_int), ("n_tokens", C.c_int), ("n_heads", C.c_int),
+                ("max_q", C.c_int), ("max_pages", C.c_int), ("window", C.c_int), ("scale", C.c_float), ("q", vp),
+                ("q_stride", C.c_longlong), ("out", vp), ("out_stride", C.c_longlong), ("page_table", vp),
+                ("kv_len", vp), ("q_start", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t), ("err", vp)]
+
+
+class ptc_sample_args(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("rows", C.c_int), ("vocab", C.c_int), ("logits", vp), ("stride", C.c_longlong),
+                ("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp), ("u", vp), ("tokens", vp)]
+
+
 MATVEC_FN = C.CFUNCTYPE(None, f32p, f32p, f32p, C.c_int, C.c_int)
 
 
@@ -238,6 +276,11 @@ def declare(L):
     _sig(L, "ptc_graph_launch", None, vp)
     _sig(L, "ptc_graph_destroy", None, vp)
     _sig(L, "ptc_d2d", None, vp, vp, vp, C.c_size_t)
+    _sig(L, "ptc_plan_pages", C.c_int, P(ptc_pages_args), vp)
+    _sig(L, "ptc_kv_append", C.c_int, P(ptc_append_args), vp)
+    _sig(L, "ptc_rope_table", C.c_int, vp, C.c_int, C.c_int, vp)
+    _sig(L, "ptc_paged_attention", C.c_int, P(ptc_attn_args), vp)
+    _sig(L, "ptc_sample_tokens", C.c_int, P(ptc_sample_args), vp)
     return declare_text(L)
 
 

@@ -1764,11 +1764,13 @@ __global__ void k_rope_table(float2 *t, int seq, int hd) {
     }
 }
 
-void build_rope_table(float2 *t, int seq, int hd, cudaStream_t s) {
+cudaError_t launch_rope_table(float2 *t, int seq, int hd, cudaStream_t s) {
     const int n = seq * (hd / 2);
     k_rope_table<<<(n + 255) / 256, 256, 0, s>>>(t, seq, hd);
-    PTC_CHECK(cudaGetLastError());
+    return cudaGetLastError();
 }
+
+void build_rope_table(float2 *t, int seq, int hd, cudaStream_t s) { PTC_CHECK(launch_rope_table(t, seq, hd, s)); }
 
 int decode_attn_limits_ok(int hd, int chunk, int n_chunks) {
     // scores: 4 threads per position, <= 4 float4 each (hd <= 64); values:

@@ -29,6 +29,8 @@ void launch_layers(const DecodeModel &m, int l0, int l1, bool from_embedding, in
 int decode_ffn_rows(int dim, int hidden, int n_sm);
 void launch_block(const DecodeModel &m, int kind, int l, int n_sm, cudaStream_t s);
 int decode_attn_stage(int dim, int nh, int nkv, int seq);
+// The decoder's RoPE table; the launch form reports a failure, the other aborts on it.
+cudaError_t launch_rope_table(float2 *t, int seq, int hd, cudaStream_t s);
 void build_rope_table(float2 *t, int seq, int hd, cudaStream_t s);
 void transpose_w2(const DecodeModel &m, float *w2t, cudaStream_t s);
 // host_next: pinned host word that also receives the argmax (or null).
