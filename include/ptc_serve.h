@@ -42,9 +42,9 @@ enum {
     PTC_SERVE_ERR_INDEX = 16    /* a page, slot or position out of range */
 };
 
-/* ---- page tables and slot maps -------------------------------------------- */
+#define PTC_SERVE_MAX_SEQS 4096   /* sequences of one call */
 
-#define PTC_PLAN_MAX_SEQS 8192
+/* ---- page tables and slot maps -------------------------------------------- */
 
 /* One step of n_seqs sequences, of which sequence r holds past_len[r] tokens
  * in the first ceil(past_len[r] / page_size) pages of its page_table row and
@@ -65,7 +65,7 @@ enum {
  * -1, q_start is zero everywhere, kv_len = past_len and *pages_used = 0, so
  * that the operators below do nothing. No output may overlap another array. */
 typedef struct {
-    int n_seqs;             /* 0 .. PTC_PLAN_MAX_SEQS */
+    int n_seqs;             /* 0 .. PTC_SERVE_MAX_SEQS */
     int page_size;          /* tokens per page, >= 1 */
     int max_pages;          /* columns of page_table, >= 1 */
     int max_tokens;         /* entries of slots and positions */
@@ -138,7 +138,8 @@ int ptc_rope_table(float *table, int n_pos, int head_dim, void *stream);
 /* ---- attention of new tokens over the paged cache ----------------------------- */
 
 /* A workspace of this size serves every ptc_paged_attention call. The caller
- * zeroes it once; each call leaves its flags zero again. Calls that may run
+ * zeroes it once; each call leaves the flags at its front (4096 bytes) zero
+ * again. Calls that may run
  * at the same time need workspaces of their own, and so do two graphs that
  * may be replayed at the same time. */
 #define PTC_ATTN_WORKSPACE_BYTES ((size_t)64 << 20)
@@ -160,7 +161,7 @@ int ptc_rope_table(float *table, int n_pos, int head_dim, void *stream);
  * bytes. The same inputs give the same bits in every call. */
 typedef struct {
     ptc_paged_cache cache;
-    int n_seqs;
+    int n_seqs;             /* 0 .. PTC_SERVE_MAX_SEQS */
     int n_tokens;           /* rows of q and out */
     int n_heads;            /* a multiple of n_kv_heads */
     int max_q;

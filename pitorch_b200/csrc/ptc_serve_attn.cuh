@@ -1,0 +1,183 @@
+// ptc_serve_attn.cuh -- how paged attention is cut into work (shared by its
+// kernels).
+//
+// An item is (sequence, K/V head, row tile): the query heads of one K/V head
+// are packed as rows, row i = token i / group, head i % group, and a tile has
+// a fixed number of them, so a key that is read serves them all. An item's
+// work is counted in units of a fixed number of keys, and the units of all
+// items, laid end to end, are cut into one equal range per CTA. So one long
+// sequence among short ones, or one sequence alone, loads the whole GPU
+// evenly, whatever the lengths are, and these are only known on the device.
+//
+// A CTA that has part of an item writes its running maximum, sum and
+// unnormalised output to the workspace. The last one to arrive at the item's
+// counter adds the parts in their order (the result does not depend on who is
+// last), writes the rows and sets the counter back to zero. Only a CTA's
+// first and last item can be partial, so two slots per CTA are enough: slot
+// 2c holds a part that began before CTA c, slot 2c + 1 one that begins in it.
+#pragma once
+
+#include "ptc_serve.cuh"
+
+namespace ptc {
+
+constexpr int ATTN_MAX_SEQS = PTC_SERVE_MAX_SEQS;
+constexpr int ATTN_FLAG_BYTES = 4096;   // counters at the front of the workspace, one per CTA
+constexpr float LOG2E = 1.4426950408889634f;
+
+// One sequence as the kernels use it; bad lengths give no rows.
+struct AttnSeq {
+    int q0;     // first row of q and out
+    int n;      // rows (tokens)
+    int pos0;   // position of the first one (may be negative)
+    int cap;    // cached positions that the page table can hold
+    int bad;
+};
+
+__device__ __forceinline__ AttnSeq attn_seq(const ptc_attn_args &a, int r) {
+    AttnSeq s;
+    s.q0 = a.q_start[r];
+    const int q1 = a.q_start[r + 1], kv = a.kv_len[r];
+    const long long room = (long long)a.max_pages * a.cache.page_size;
+    s.n = q1 - s.q0;
+    s.bad = 0;
+    s.pos0 = kv - s.n;
+    s.cap = kv;
+    if (s.q0 < 0 || q1 < s.q0 || q1 > a.n_tokens || kv < 0) s.bad = PTC_SERVE_ERR_LENGTH, s.n = 0;
+    else if (kv > room) s.bad = PTC_SERVE_ERR_LENGTH, s.cap = (int)room;
+    return s;
+}
+
+// The keys [lo, hi) that rows [i0, i1) of a sequence see (i = token * group + head).
+__device__ __forceinline__ void attn_keys(const AttnSeq &s, int group, int window, int i0, int i1, int &lo, int &hi) {
+    hi = min(s.pos0 + (i1 - 1) / group + 1, s.cap);
+    lo = window > 0 ? max(0, s.pos0 + i0 / group - window + 1) : 0;
+}
+
+// Units of row tile m of a sequence: one at least, so that rows that see nothing are written.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int attn_units(const AttnSeq &s, int group, int window, int m) {
+    int lo, hi;
+    attn_keys(s, group, window, m * ROWS, min(s.n * group, (m + 1) * ROWS), lo, hi);
+    return hi > lo ? (hi + KEYS - 1) / KEYS - lo / KEYS : 1;
+}
+
+// pre[r] = units of one K/V head of the sequences before r, by all THREADS
+// threads of the CTA; pre[n_seqs] is the total. scratch: THREADS / 32 ints. A
+// total past 2^31 / heads leaves nothing to do (LENGTH).
+template <int ROWS, int KEYS, int THREADS>
+__device__ void attn_prefix(const ptc_attn_args &a, int group, int *pre, long long *scratch) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_seqs;
+    const int per = (n + THREADS - 1) / THREADS, r0 = min(n, tid * per);
+    long long sum = 0;
+    int bad = 0;
+    for (int k = 0; k < per; k++) {
+        const int r = r0 + k;
+        const bool mine = r < n;
+        AttnSeq s = {0, 0, 0, 0, 0};
+        if (mine) s = attn_seq(a, r);
+        bad |= s.bad;
+        const long long rows = (long long)s.n * group;
+        const int tiles = (int)((rows + ROWS - 1) / ROWS);
+        long long u = 0;
+        if (tiles <= 8)
+            for (int m = 0; m < tiles; m++) u += attn_units<ROWS, KEYS>(s, group, a.window, m);
+        // a long chunk's tiles are counted by the whole warp
+        unsigned many = __ballot_sync(0xffffffffu, tiles > 8);
+        while (many) {
+            const int src = __ffs(many) - 1;
+            many &= many - 1;
+            AttnSeq b;
+            b.n = __shfl_sync(0xffffffffu, s.n, src);
+            b.pos0 = __shfl_sync(0xffffffffu, s.pos0, src);
+            b.cap = __shfl_sync(0xffffffffu, s.cap, src);
+            const int all = __shfl_sync(0xffffffffu, tiles, src);
+            long long v = 0;
+            for (int m = lane; m < all; m += 32) v += attn_units<ROWS, KEYS>(b, group, a.window, m);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == src) u = v;
+        }
+        if (mine) pre[r] = (int)min(u, (long long)INT32_MAX);
+        sum += u;
+    }
+    if (bad && blockIdx.x == 0) serve_err(a.err, bad);
+    long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+    }
+    if (lane == 31) scratch[warp] = inc;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) {
+        if (w == warp) before = total;
+        total += scratch[w];
+    }
+    if (total > INT32_MAX / a.cache.n_kv_heads) {
+        if (tid == 0 && blockIdx.x == 0) serve_err(a.err, PTC_SERVE_ERR_LENGTH);
+        total = before = sum = inc = 0;
+        for (int k = 0; k < per; k++)
+            if (r0 + k < n) pre[r0 + k] = 0;
+    }
+    int at = (int)(before + inc - sum);
+    for (int k = 0; k < per; k++)
+        if (r0 + k < n) {
+            const int u = pre[r0 + k];
+            pre[r0 + k] = at;
+            at += u;
+        }
+    if (tid == 0) pre[n] = (int)total;
+    __syncthreads();
+}
+
+// One item and the part of it that a CTA has.
+struct AttnItem {
+    AttnSeq s;
+    int r, head;        // sequence, K/V head
+    int i0, i1;         // its rows
+    int lo, hi;         // the keys they see
+    int first, units;   // its first unit among all, and how many it has
+};
+
+// The item that holds unit u. All threads of a CTA get the same.
+template <int ROWS, int KEYS>
+__device__ AttnItem attn_find(const ptc_attn_args &a, int group, const int *pre, int u) {
+    AttnItem it;
+    const int heads = a.cache.n_kv_heads;
+    int lo = 0, hi = a.n_seqs;   // last r with pre[r] * heads <= u (sequences without units share their start)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] * heads <= u) lo = mid;
+        else hi = mid;
+    }
+    it.r = lo;
+    const int per = pre[lo + 1] - pre[lo], in = u - pre[lo] * heads;
+    it.head = in / per;
+    it.s = attn_seq(a, lo);
+    int rest = in - it.head * per, m = 0, n;
+    for (;; m++) {
+        n = attn_units<ROWS, KEYS>(it.s, group, a.window, m);
+        if (rest < n) break;
+        rest -= n;
+    }
+    it.i0 = m * ROWS;
+    it.i1 = min(it.s.n * group, (m + 1) * ROWS);
+    attn_keys(it.s, group, a.window, it.i0, it.i1, it.lo, it.hi);
+    it.first = u - rest;
+    it.units = n;
+    return it;
+}
+
+// CTA c of C has units [first(c), first(c + 1)) of `total`; owner(u) is the one that has unit u.
+__device__ __forceinline__ int attn_first(int c, int C, int total) { return (int)((long long)c * total / C); }
+__device__ __forceinline__ int attn_owner(int u, int C, int total) { return (int)((((long long)u + 1) * C - 1) / total); }
+
+// Element t of a sequence: its offset in the cache without the head's share, or -1.
+__device__ __forceinline__ long long attn_cell(const ptc_attn_args &a, int page, int off) {
+    return (unsigned)page < (unsigned)a.cache.n_pages ? page * a.cache.page_stride + off * a.cache.token_stride : -1;
+}
+
+}  // namespace ptc

@@ -24,7 +24,7 @@ const char *check_cache(const ptc_paged_cache &c) {
 // Page tables and slot maps: two exclusive scans over the sequences (new
 // tokens and new pages), then one search per token and per new page.
 //
-// One kernel. Every CTA scans all sequences itself (at most 8192, from L2) --
+// One kernel. Every CTA scans all sequences itself (at most 4096, from L2) --
 // a few hundred nanoseconds, against a second launch or a grid barrier of
 // more than a microsecond -- so each also knows whether the step fits before
 // it writes anything. A table entry is read only where cached tokens lie and
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(AP_THREADS) k_kv_append(ptc_append_args a, int
 extern "C" int ptc_plan_pages(const ptc_pages_args *p, void *stream) {
     if (!p) SERVE_REFUSE("no arguments");
     const ptc_pages_args a = *p;
-    if (a.n_seqs < 0 || a.n_seqs > PTC_PLAN_MAX_SEQS) SERVE_REFUSE("n_seqs %d is outside 0..%d", a.n_seqs, PTC_PLAN_MAX_SEQS);
+    if (a.n_seqs < 0 || a.n_seqs > PTC_SERVE_MAX_SEQS) SERVE_REFUSE("n_seqs %d is outside 0..%d", a.n_seqs, PTC_SERVE_MAX_SEQS);
     if (a.page_size < 1 || a.max_pages < 1 || a.max_tokens < 0 || a.n_free < 0 || a.n_pages < 1)
         SERVE_REFUSE("bad size (page_size %d, max_pages %d, max_tokens %d, n_free %d, n_pages %d)", a.page_size,
                      a.max_pages, a.max_tokens, a.n_free, a.n_pages);
