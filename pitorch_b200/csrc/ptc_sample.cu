@@ -1,9 +1,69 @@
 // ptc_sample.cu -- sampling of the next tokens on the GPU (include/ptc_serve.h).
+//
+// A cluster of 1 to 8 CTAs per row; each holds its slice of the logits in
+// shared memory, so the row is read from memory once. Nothing is sorted. The
+// kept tokens are those whose (value, lowest index first) key is at or above
+// one threshold, which is found by counting:
+//
+//  1. the maximum;
+//  2. a histogram of the logits by their distance from it (4096 bins of equal
+//     width down to where a weight is zero), exchanged through distributed
+//     shared memory. The bin that holds the k-th largest is collected and its
+//     few members ranked: the threshold of top_k;
+//  3. top_p: a bin's mass lies between its count times its lowest and highest
+//     weight, 0.8% apart, so the counts alone bracket the bins in which the
+//     mass can reach top_p times the total. The mass before the bracket is
+//     summed exactly; inside it, a second histogram of exact masses (1024
+//     bins) or, where there are few members, their ranking finds the last one
+//     kept;
+//  4. min_p is a comparison with the weight, and the token is found from the
+//     kept sums of the CTAs, of their warps and of one warp's elements.
+//
+// Where a bin has too many members to be ranked (equal logits by the
+// thousand), the threshold is bisected instead.
+//
+// Weights are integers in units of 2^-43 of the largest, so every sum is
+// exact, the order of the atomics has no effect, and the same row gives the
+// same token in any batch. They are computed in 64-bit arithmetic (2^y by a
+// table of 32 and a polynomial of degree 5, relative error below 2^-45): the
+// running sum of 10^5 weights has to be exact to far better than the weight
+// of one token, which 32-bit exponentials do not give.
+#include <cooperative_groups.h>
+
 #include "ptc_serve.cuh"
 
 namespace ptc {
+namespace cg = cooperative_groups;
 
-constexpr int SM_THREADS = 1024;
+constexpr int SP_THREADS = 512;
+constexpr int SP_WARPS = SP_THREADS / 32;
+constexpr int SP_BINS = 4096;     // of the first histogram; the last one holds what has no weight
+constexpr int SP_BINS2 = 1024;    // of the second
+constexpr int SP_LIST = 1024;     // members that are ranked
+constexpr int SP_FEW = 256;       // ... without a second histogram
+constexpr int SP_PER = SP_BINS / SP_THREADS;
+constexpr int SP_SLICE = 16384;   // logits of a CTA, while 8 of them hold the row
+constexpr float SP_RANGE = 44.f;  // weights below 2^-44 are zero
+typedef unsigned long long u64;
+constexpr double SP_ONE = 8796093022208.0;   // 2^43
+
+struct alignas(16) SampleShared {
+    unsigned hist[SP_BINS];
+    // the second histogram (sums of the weights' low, middle and high 15 bits),
+    // or a list of all CTAs' members with their weights
+    union {
+        unsigned mass[3][SP_BINS2];
+        struct {
+            u64 key[SP_LIST], w[SP_LIST];
+        } all;
+    };
+    u64 list[SP_LIST];   // this CTA's members
+    unsigned n_list[2];
+    double table[32];    // 2^(j/32)
+    u64 part[SP_WARPS], box[6], step[2];   // sums of warps; values that the other CTAs read
+    u64 found;
+    int bin, above, in_bin, b_lo, b_hi, range_n;
+};
 
 // A logit as the rules see it: NaN counts as -inf, and -0 as 0, so that equal
 // values have equal keys.
@@ -12,164 +72,534 @@ __device__ __forceinline__ float logit(T v) {
     const float x = Elem<T>::up(v);
     return x != x ? -INFINITY : x + 0.0f;
 }
-
-// Weights are held as integers in units of 2^-43 of the largest one: their
-// sums are exact in any order, and 2^18 of them stay below 2^61.
-__device__ __forceinline__ unsigned long long weight(float x, float top, double rt) {
-    if (x == top) return 1ull << 43;
-    if (x == -INFINITY) return 0;
-    return (unsigned long long)__double2ll_rn(exp(((double)x - (double)top) * rt) * 8796093022208.0);
+__device__ __forceinline__ float key_value(u64 key) {
+    const uint32_t k = (uint32_t)(key >> 32);
+    return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
-__device__ unsigned long long block_sum(unsigned long long v, unsigned long long *sh) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// How a row's logits become bins and weights.
+struct Weigh {
+    float top, scale;   // bins per unit of distance
+    double c, topc;     // log2(e) / temperature, and times the maximum
+    const double *table;
+
+    __device__ float place(float x) const { return x == top ? 0.f : (top - x) * scale; }
+    __device__ static int bin(float f) { return f < (float)(SP_BINS - 1) ? (int)f : SP_BINS - 1; }
+    // 2^y for y = (x - top) log2(e) / temperature: y = n/32 + r, 2^(n/32) from
+    // the table and the exponent, 2^r by its series (ln 2)^i / i!
+    __device__ u64 weight(float x) const {
+        if (x == top) return 1ull << 43;
+        if (!(place(x) < (float)(SP_BINS - 1))) return 0;
+        const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the rounded integer
+        const double y = fma((double)x, c, -topc), t = fma(y, 32.0, magic);
+        const int n = __double2loint(t);
+        const double r = fma(t - magic, -1.0 / 32.0, y);
+        double p = 1.3333558146428443e-3;
+        p = fma(p, r, 9.618129107628477e-3);
+        p = fma(p, r, 5.550410866482158e-2);
+        p = fma(p, r, 2.402265069591007e-1);
+        p = fma(p, r, 6.931471805599453e-1);
+        p = fma(p, r, 1.0) * table[n & 31];
+        p = __hiloint2double(__double2hiint(p) + (((n >> 5) + 43) << 20), __double2loint(p));
+        return (u64)__double_as_longlong(p + 4503599627370496.0) & ((1ull << 52) - 1);
+    }
+};
+
+__device__ __forceinline__ u64 warp_add(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ u64 warp_top(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// The CTA's sum of v, in every thread.
+__device__ u64 block_add(u64 v, u64 *part) {
+    v = warp_add(v);
     __syncthreads();
-    if (lane == 0) sh[warp] = v;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    unsigned long long t = 0;
-    for (int w = 0; w < SM_THREADS / 32; w++) t += sh[w];
+    u64 t = 0;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) t += part[w];
     return t;
 }
 
-// One CTA per row: the thresholds by bisection over the ordered keys.
+// The sum of `box` over the cluster (after a barrier of the cluster).
+__device__ u64 peers_sum(cg::cluster_group &cl, u64 *box) {
+    u64 t = 0;
+    for (unsigned q = 0; q < cl.num_blocks(); q++) t += *cl.map_shared_rank(box, q);
+    return t;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(SM_THREADS) k_sample(ptc_sample_args a) {
-    __shared__ unsigned long long sh[SM_THREADS / 32];
-    const int row = blockIdx.x, tid = threadIdx.x, V = a.vocab;
-    const T *x = (const T *)a.logits + row * a.stride;
-    const float temp = a.temperature ? a.temperature[row] : 1.0f;
-    const bool greedy = !(temp > 0.0f);
+struct SampleRow {
+    SampleShared &sh;
+    cg::cluster_group &cl;
+    const T *x;     // this CTA's slice in shared memory
+    int n, first;   // its length and the index of its first logit
+    Weigh wt;
+    int turn;       // the slot of sh.step that the next sum takes: the other CTAs may still read the last one
 
-    unsigned long long best = 0;
-    for (int i = tid; i < V; i += SM_THREADS) best = max(best, argmax_key(logit(x[i]), i));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if ((tid & 31) == 0) sh[tid >> 5] = best;
-    __syncthreads();
-    for (int w = 0; w < SM_THREADS / 32; w++) best = max(best, sh[w]);
-    const uint32_t top_key = (uint32_t)(best >> 32);
-    const int first = argmax_key_index(best);
-    const float top = logit(x[first]);
-    if (top == -INFINITY || greedy) {
-        if (tid == 0) a.tokens[row] = top == -INFINITY ? -1 : first;
-        return;
-    }
-    const double rt = 1.0 / (double)temp;
+    __device__ u64 key(float v, int i) const { return argmax_key(v, first + i); }
 
-    // top_k: the largest key with at least k keys at or above it
-    const int k = a.top_k ? a.top_k[row] : 0;
-    uint32_t cut = 0;
-    unsigned long long ties = V;   // how many of the elements equal to `cut` are kept
-    if (k > 0 && k < V) {
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t c = cut | (1u << bit);
-            unsigned long long n = 0;
-            for (int i = tid; i < V; i += SM_THREADS) n += float_key(logit(x[i])) >= c;
-            if (block_sum(n, sh) >= (unsigned long long)k) cut = c;
-        }
-        unsigned long long above = 0;
-        for (int i = tid; i < V; i += SM_THREADS) above += float_key(logit(x[i])) > cut;
-        ties = k - block_sum(above, sh);
-    }
-    // mass above a key, and of the kept elements that equal `cut`
-    auto mass_above = [&](uint32_t key) {
-        unsigned long long m = 0;
-        for (int i = tid; i < V; i += SM_THREADS) {
+    // Sum over the cluster of f(value, key), a barrier of the cluster in it.
+    template <typename F>
+    __device__ u64 sum(F f) {
+        u64 s = 0;
+        for (int i = threadIdx.x; i < n; i += SP_THREADS) {
             const float v = logit(x[i]);
-            if (float_key(v) > key) m += weight(v, top, rt);
+            s += f(v, key(v, i));
         }
-        return block_sum(m, sh);
-    };
-    auto key_value = [](uint32_t key) { return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key); };
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
-    if (p < 1.0f) {
-        unsigned long long total = mass_above(cut);
-        unsigned long long equal = 0;
-        for (int i = tid; i < V; i += SM_THREADS) equal += float_key(logit(x[i])) == cut;
-        equal = min(block_sum(equal, sh), ties);
-        if (equal) total += equal * weight(key_value(cut), top, rt);
-        const double want = (double)p * (double)total;
-        uint32_t lo = cut, hi = top_key;   // the lowest key with less than `want` above it
+        s = block_add(s, sh.part);
+        u64 *slot = &sh.step[turn];
+        turn ^= 1;
+        if (threadIdx.x == 0) *slot = s;
+        cl.sync();
+        return peers_sum(cl, slot);
+    }
+
+    // The k-th largest key, by bisection.
+    __device__ u64 bisect_count(u64 k, u64 top) {
+        u64 lo = 0, hi = top;   // the largest key with at least k at or above it
         while (lo < hi) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            if ((double)mass_above(mid) < want) hi = mid;
+            const u64 mid = lo + (hi - lo + 1) / 2;
+            if (sum([&](float, u64 e) { return (u64)(e >= mid); }) >= k) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
+    // The lowest key at or above `floor` with less than `want` above it.
+    __device__ u64 bisect_mass(double want, u64 floor, u64 top) {
+        u64 lo = floor, hi = top;
+        while (lo < hi) {
+            const u64 mid = lo + (hi - lo) / 2;
+            const u64 m = sum([&](float v, u64 e) { return e > mid ? wt.weight(v) : 0; });
+            if ((double)m < want) hi = mid;
             else lo = mid + 1;
         }
-        const unsigned long long above = mass_above(lo), w = weight(key_value(lo), top, rt);
-        if (lo > cut) {
-            unsigned long long n = 0;
-            for (int i = tid; i < V; i += SM_THREADS) n += float_key(logit(x[i])) == lo;
-            ties = block_sum(n, sh);
-        }
-        // of the equal ones, those with less than `want` before them (one at least where it is the maximum)
-        unsigned long long j = 0;
-        while (j < ties && (double)(above + j * w) < want && w) j++;
-        if (w) ties = j;
-        if (lo == top_key && ties == 0) ties = 1;
-        cut = lo;
+        return lo;
     }
-    const float mp = a.min_p ? a.min_p[row] : 0.0f;
-    // rank among the equal ones and running mass, in index order
-    unsigned long long done_ties = 0;
-    unsigned long long total = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        unsigned long long run = 0, want = 0;
-        if (pass) {
-            const float u = a.u[row];
-            const double r = floor((double)u * (double)total);
-            want = r > 0 ? (unsigned long long)r : 0;
-            if (want >= total) want = total - 1;
-        }
-        done_ties = 0;
-        __shared__ int found;
-        if (tid == 0) found = -1;
+
+    // Collects the keys that `in` picks and, over the slice, the sum of `add`;
+    // one barrier of the cluster. Every CTA then has all of them in sh.all.key
+    // (their number is returned; more than SP_LIST: nothing to use). The two
+    // calls of a row use a list and a box each, as the other CTAs may still read
+    // the first when the second begins; the second's list takes the place of the
+    // first histogram, which everyone has read by then.
+    template <typename In, typename Add>
+    __device__ int collect(In in, Add add, u64 &total, int box, int second) {
+        static_assert(sizeof(sh.hist) >= sizeof(sh.list), "the second list fits");
+        u64 *list = second ? (u64 *)sh.hist : sh.list;
+        unsigned *count = &sh.n_list[second];
+        if (threadIdx.x == 0) *count = 0;
         __syncthreads();
-        for (int base = 0; base < V; base += SM_THREADS) {
-            const int i = base + tid;
-            const float v = i < V ? logit(x[i]) : -INFINITY;
-            const uint32_t key = float_key(v);
-            const bool tie = i < V && key == cut;
-            // exclusive rank of this tie in the chunk
-            const unsigned mask = __ballot_sync(0xffffffffu, tie);
-            __syncthreads();
-            if ((tid & 31) == 0) sh[tid >> 5] = __popc(mask);
-            __syncthreads();
-            unsigned long long before = 0, all = 0;
-            for (int w = 0; w < SM_THREADS / 32; w++) {
-                if (w == (tid >> 5)) before = all;
-                all += sh[w];
+        u64 s = 0;
+        for (int i = threadIdx.x; i < n; i += SP_THREADS) {
+            const float v = logit(x[i]);
+            const u64 e = key(v, i);
+            const float f = wt.place(v);
+            if (in(e, f)) {
+                const unsigned at = atomicAdd(count, 1u);
+                if (at < SP_LIST) list[at] = e;
+            } else {
+                s += add(v, e, f);
             }
-            const unsigned long long rank = done_ties + before + __popc(mask & ((1u << (tid & 31)) - 1));
-            done_ties += all;
-            unsigned long long w = 0;
-            if (i < V && (key > cut || (tie && rank < ties))) {
-                w = weight(v, top, rt);
-                if ((double)w < (double)mp * 8796093022208.0) w = 0;
+        }
+        s = block_add(s, sh.part);
+        if (threadIdx.x == 0) sh.box[box] = s;
+        cl.sync();
+        total = peers_sum(cl, &sh.box[box]);
+        int at = 0;
+        for (unsigned q = 0; q < cl.num_blocks(); q++) {
+            const int c = (int)min(*cl.map_shared_rank(count, q), (unsigned)SP_LIST + 1);
+            const u64 *from = cl.map_shared_rank(list, q);
+            if (at + c <= SP_LIST)
+                for (int i = threadIdx.x; i < c; i += SP_THREADS) sh.all.key[at + i] = from[i];
+            at = min(at + c, SP_LIST + 1);
+        }
+        __syncthreads();
+        return at;
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int slice) {
+    extern __shared__ __align__(16) char sp_smem[];
+    SampleShared &sh = *(SampleShared *)sp_smem;
+    cg::cluster_group cl = cg::this_cluster();
+    const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank(), row = blockIdx.x / CL;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int first = min(a.vocab, rank * slice), n = min(slice, a.vocab - first);
+
+    // The slice into shared memory, at the same offset from a 16-byte boundary as in memory.
+    const T *src = (const T *)a.logits + row * a.stride + first;
+    constexpr int N = Vec16<T>::N;
+    const int shift = (int)(((uintptr_t)src & 15) / sizeof(T));
+    T *x = (T *)(sp_smem + sizeof(SampleShared)) + shift;
+    u64 best = 0;
+    {
+        float top = -INFINITY;
+        int at = -1;
+        for (int v = tid; v * N < n + shift; v += SP_THREADS) {
+            const int i0 = v * N - shift;
+            if (i0 >= 0 && i0 + N <= n) {
+                const Vec16<T> e = *(const Vec16<T> *)(src + i0);
+                *(Vec16<T> *)(x + i0) = e;
+#pragma unroll
+                for (int k = 0; k < N; k++) {
+                    const float f = logit(e.e[k]);
+                    if (f > top || at < 0) top = f, at = i0 + k;
+                }
+            } else {
+                for (int k = max(0, -i0); k < N && i0 + k < n; k++) {
+                    const T e = src[i0 + k];
+                    x[i0 + k] = e;
+                    const float f = logit(e);
+                    if (f > top || at < 0) top = f, at = i0 + k;
+                }
             }
-            unsigned long long inc = w;
+        }
+        if (at >= 0) best = argmax_key(top, first + at);
+    }
+    for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.hist[i] = 0;
+    if (tid < 32) sh.table[tid] = exp2((double)tid / 32.0);
+    best = warp_top(best);
+    if (lane == 0) sh.part[warp] = best;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 0; w < SP_WARPS; w++) best = max(best, sh.part[w]);
+        sh.box[0] = best;
+    }
+    cl.sync();
+    best = 0;
+    for (int q = 0; q < CL; q++) best = max(best, *cl.map_shared_rank(&sh.box[0], q));
+
+    const float temp = a.temperature ? a.temperature[row] : 1.0f, top = key_value(best);
+    if (top == -INFINITY || !(temp > 0.0f)) {
+        if (tid == 0 && rank == 0) a.tokens[row] = top == -INFINITY ? -1 : argmax_key_index(best);
+        cl.sync();   // nobody reads a CTA's shared memory after it has left
+        return;
+    }
+    const double c = 1.4426950408889634 / (double)temp;
+    const Weigh wt = {top, (float)((SP_BINS - 1) / SP_RANGE * c), c, (double)top * c, sh.table};
+    SampleRow<T> R = {sh, cl, x, n, first, wt, 0};
+    const int want_k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f;
+    const bool by_k = want_k > 0 && want_k < a.vocab, by_p = p < 1.0f;
+    u64 floor_key = 0;   // tokens with a key at or above it are kept
+
+    if (by_k || by_p) {
+        // counts of the bins; with top_p alone, the mass of the row
+        u64 mass = 0;
+        for (int i = tid; i < n; i += SP_THREADS) {
+            const float v = logit(x[i]);
+            const int b = Weigh::bin(wt.place(v));
+            if (b < SP_BINS - 1) {
+                atomicAdd(&sh.hist[b], 1u);
+                if (!by_k) mass += wt.weight(v);
+            }
+        }
+        mass = block_add(mass, sh.part);
+        if (tid == 0) {
+            sh.box[1] = mass;
+            sh.bin = SP_BINS - 1;
+        }
+        cl.sync();
+        u64 total = peers_sum(cl, &sh.box[1]);
+        int cnt[SP_PER], mine = 0;
+#pragma unroll
+        for (int i = 0; i < SP_PER; i++) cnt[i] = 0;
+        for (int q = 0; q < CL; q++) {
+            const uint4 *h = (const uint4 *)(cl.map_shared_rank(sh.hist, q) + tid * SP_PER);
+#pragma unroll
+            for (int i = 0; i < SP_PER / 4; i++) {
+                const uint4 u = h[i];
+                cnt[4 * i] += u.x;
+                cnt[4 * i + 1] += u.y;
+                cnt[4 * i + 2] += u.z;
+                cnt[4 * i + 3] += u.w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < SP_PER; i++) mine += cnt[i];
+        if (by_k) {
+            int inc = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long y = __shfl_up_sync(0xffffffffu, inc, o);
-                if ((tid & 31) >= o) inc += y;
+                const int y = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += y;
             }
             __syncthreads();
-            if ((tid & 31) == 31) sh[tid >> 5] = inc;
+            if (lane == 31) sh.part[warp] = inc;
             __syncthreads();
-            unsigned long long pre = 0, sum = 0;
-            for (int q = 0; q < SM_THREADS / 32; q++) {
-                if (q == (tid >> 5)) pre = sum;
-                sum += sh[q];
+            int before = inc - mine;
+            for (int w = 0; w < warp; w++) before += (int)sh.part[w];
+#pragma unroll
+            for (int i = 0; i < SP_PER; i++) {   // the bin in which the count reaches k
+                if (before < want_k && before + cnt[i] >= want_k) sh.bin = tid * SP_PER + i, sh.above = before, sh.in_bin = cnt[i];
+                before += cnt[i];
             }
-            const unsigned long long c1 = run + pre + inc, c0 = c1 - w;
-            if (pass && w && c0 <= want && want < c1) found = i;
-            run += sum;
+            __syncthreads();
+            const int bk = sh.bin;
+            if (bk < SP_BINS - 1) {   // else all that has weight is among the k largest
+                const int rest = want_k - sh.above;   // of the bin's members
+                u64 over = 0;
+                const int m = sh.in_bin <= SP_LIST ? R.collect([&](u64, float f) { return Weigh::bin(f) == bk; },
+                                                               [&](float v, u64, float f) { return by_p && Weigh::bin(f) < bk ? wt.weight(v) : 0; }, over, 2, 0)
+                                                   : SP_LIST + 1;
+                if (m <= SP_LIST) {
+                    for (int i = tid; i < m; i += SP_THREADS) {
+                        const u64 e = sh.all.key[i];
+                        int rank_ = 0;
+                        for (int j = 0; j < m; j++) rank_ += sh.all.key[j] > e;
+                        if (rank_ == rest - 1) sh.found = e;
+                    }
+                    __syncthreads();
+                    floor_key = sh.found;
+                    if (by_p) {
+                        u64 w = 0;
+                        for (int i = tid; i < m; i += SP_THREADS)
+                            if (sh.all.key[i] >= floor_key) w += wt.weight(key_value(sh.all.key[i]));
+                        total = over + block_add(w, sh.part);
+                    }
+                } else {
+                    floor_key = R.bisect_count(want_k, best);
+                    if (by_p) total = R.sum([&](float v, u64 e) { return e >= floor_key ? wt.weight(v) : 0; });
+                }
+                // the counts that are left for top_p
+#pragma unroll
+                for (int i = 0; i < SP_PER; i++) {
+                    const int b = tid * SP_PER + i;
+                    if (b == bk) cnt[i] = rest;
+                    if (b > bk) cnt[i] = 0;
+                }
+            } else if (by_p) {
+                total = R.sum([&](float v, u64) { return wt.weight(v); });
+            }
         }
-        if (!pass) total = run;
-        __syncthreads();
-        if (pass && tid == 0) a.tokens[row] = found;
+        if (by_p) {
+            const double want = (double)p * (double)total;
+            u64 kept = best;   // the lowest key that is kept; the largest one always is
+            if (want > 0) {
+                // bracket from the counts: bins whose mass can hold the border
+                const float q = SP_RANGE / (SP_BINS - 1), goal = (float)(want / SP_ONE);
+                float low = 0.f, high = 0.f;
+#pragma unroll
+                for (int i = 0; i < SP_PER; i++) {
+                    const float b = (float)(tid * SP_PER + i);
+                    low += cnt[i] * exp2f(-(b + 1.01f) * q);
+                    high += cnt[i] * exp2f(-(b - 0.01f) * q);
+                }
+                float il = low, ih = high;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float y = __shfl_up_sync(0xffffffffu, il, o), z = __shfl_up_sync(0xffffffffu, ih, o);
+                    if (lane >= o) il += y, ih += z;
+                }
+                float2 *fp = (float2 *)sh.part;
+                __syncthreads();
+                if (tid == 0) sh.b_lo = SP_BINS - 2, sh.b_hi = SP_BINS - 2, sh.range_n = 0;
+                if (lane == 31) fp[warp] = make_float2(il, ih);
+                __syncthreads();
+                float bl = il - low, bh = ih - high;
+                for (int w = 0; w < warp; w++) bl += fp[w].x, bh += fp[w].y;
+#pragma unroll
+                for (int i = 0; i < SP_PER; i++) {
+                    const int b = tid * SP_PER + i;
+                    bl += cnt[i] * exp2f(-((float)b + 1.01f) * q);
+                    bh += cnt[i] * exp2f(-((float)b - 0.01f) * q);
+                    if (bh * 1.0001f >= goal) atomicMin(&sh.b_lo, b);
+                    if (bl * 0.9999f >= goal) atomicMin(&sh.b_hi, b);
+                }
+                __syncthreads();
+                const int b_lo = sh.b_lo, b_hi = max(sh.b_hi, b_lo);
+                int in_range = 0;
+#pragma unroll
+                for (int i = 0; i < SP_PER; i++) {
+                    const int b = tid * SP_PER + i;
+                    if (b >= b_lo && b <= b_hi) in_range += cnt[i];
+                }
+                if (in_range) atomicAdd(&sh.range_n, in_range);
+                __syncthreads();
+                u64 over = 0;
+                int g_lo = 0, g_hi = SP_BINS2;   // the second histogram's bins that are collected
+                const float g_scale = (float)SP_BINS2 / (float)(b_hi - b_lo + 1);
+                auto sub = [&](float f) { return min(SP_BINS2 - 1, (int)((f - (float)b_lo) * g_scale)); };
+                auto inside = [&](u64 e, float f) { return e >= floor_key && Weigh::bin(f) >= b_lo && Weigh::bin(f) <= b_hi; };
+                if (sh.range_n > SP_FEW) {
+                    for (int i = tid; i < 3 * SP_BINS2; i += SP_THREADS) ((unsigned *)sh.mass)[i] = 0;
+                    __syncthreads();
+                    u64 s = 0;
+                    for (int i = tid; i < n; i += SP_THREADS) {
+                        const float v = logit(x[i]), f = wt.place(v);
+                        const u64 e = R.key(v, i);
+                        if (e < floor_key || Weigh::bin(f) > b_hi) continue;
+                        const u64 w = wt.weight(v);
+                        if (Weigh::bin(f) < b_lo) {
+                            s += w;
+                        } else {   // 15 bits at a time: the sums of 2^15 of them stay below 2^30
+                            const int g = sub(f);
+                            atomicAdd(&sh.mass[0][g], (unsigned)(w & 0x7fff));
+                            atomicAdd(&sh.mass[1][g], (unsigned)(w >> 15 & 0x7fff));
+                            atomicAdd(&sh.mass[2][g], (unsigned)(w >> 30));
+                        }
+                    }
+                    s = block_add(s, sh.part);
+                    if (tid == 0) sh.box[3] = s, sh.bin = -1;
+                    cl.sync();
+                    const u64 before = peers_sum(cl, &sh.box[3]);
+                    constexpr int PER = SP_BINS2 / SP_THREADS;
+                    u64 m[PER], sum = 0;
+#pragma unroll
+                    for (int i = 0; i < PER; i++) m[i] = 0;
+                    for (int r = 0; r < CL; r++) {
+                        const unsigned *h = cl.map_shared_rank((unsigned *)sh.mass, r) + tid * PER;
+#pragma unroll
+                        for (int i = 0; i < PER; i++) m[i] += h[i] + ((u64)h[SP_BINS2 + i] << 15) + ((u64)h[2 * SP_BINS2 + i] << 30);
+                    }
+#pragma unroll
+                    for (int i = 0; i < PER; i++) sum += m[i];
+                    u64 inc = sum;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+                        if (lane >= o) inc += y;
+                    }
+                    __syncthreads();
+                    if (lane == 31) sh.part[warp] = inc;
+                    __syncthreads();
+                    u64 at = before + inc - sum;
+                    for (int w = 0; w < warp; w++) at += sh.part[w];
+#pragma unroll
+                    for (int i = 0; i < PER; i++) {   // the bin in which the mass reaches the goal
+                        if ((double)at < want && (double)(at + m[i]) >= want) sh.bin = tid * PER + i;
+                        at += m[i];
+                    }
+                    __syncthreads();
+                    g_lo = sh.bin;
+                    g_hi = g_lo + 1;
+                }
+                // rank what is left by mass: e is kept while less than the goal is above it
+                const int m = g_lo < 0 ? SP_LIST + 1
+                                       : R.collect([&](u64 e, float f) { return inside(e, f) && sub(f) >= g_lo && sub(f) < g_hi; },
+                                                   [&](float v, u64 e, float f) {
+                                                       const int b = Weigh::bin(f);
+                                                       return e >= floor_key && (b < b_lo || (b <= b_hi && sub(f) < g_lo)) ? wt.weight(v) : 0;
+                                                   }, over, 4, by_k);
+                bool done = false;
+                if (m <= SP_LIST) {
+                    for (int i = tid; i < m; i += SP_THREADS) sh.all.w[i] = wt.weight(key_value(sh.all.key[i]));
+                    if (tid == 0) sh.found = ~0ull;
+                    __syncthreads();
+                    for (int i = tid; i < m; i += SP_THREADS) {
+                        const u64 e = sh.all.key[i];
+                        u64 above = over;
+                        for (int j = 0; j < m; j++)
+                            if (sh.all.key[j] > e) above += sh.all.w[j];
+                        if ((double)above < want) atomicMin(&sh.found, e);
+                    }
+                    __syncthreads();
+                    done = sh.found != ~0ull;
+                    if (done) kept = sh.found;
+                }
+                if (!done) kept = R.bisect_mass(want, floor_key, best);
+            }
+            floor_key = max(floor_key, kept);
+        }
     }
+
+    // The kept weights in index order: a warp has a run of the slice.
+    const float mp = a.min_p ? a.min_p[row] : 0.0f;
+    const double least = (mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE;
+    auto kept_weight = [&](int i) -> u64 {
+        const float v = logit(x[i]);
+        if (R.key(v, i) < floor_key) return 0;
+        const u64 w = wt.weight(v);
+        return (double)w < least ? 0 : w;
+    };
+    const int run = (n + SP_THREADS - 1) / SP_THREADS * 32;
+    u64 s = 0;
+    for (int i = warp * run + lane; i < min(n, (warp + 1) * run); i += 32) s += kept_weight(i);
+    s = warp_add(s);
+    __syncthreads();
+    if (lane == 0) sh.part[warp] = s;
+    __syncthreads();
+    if (tid == 0) {
+        u64 t = 0;
+        for (int w = 0; w < SP_WARPS; w++) t += sh.part[w];
+        sh.box[5] = t;
+    }
+    cl.sync();
+    u64 before = 0, total = 0, own = 0;
+    for (int q = 0; q < CL; q++) {
+        const u64 t = *cl.map_shared_rank(&sh.box[5], q);
+        if (q < rank) before += t;
+        if (q == rank) own = t;
+        total += t;
+    }
+    cl.sync();   // the others may leave
+    const double u = (double)a.u[row] * (double)total;
+    u64 goal = u > 0 ? (u < (double)total ? (u64)u : total - 1) : 0;
+    if (goal >= total) goal = total - 1;
+    if (goal < before || goal >= before + own) return;
+    goal -= before;
+    u64 at = 0;
+    int w0 = 0;   // the warp's run that holds it
+    for (; w0 < SP_WARPS - 1 && at + sh.part[w0] <= goal; w0++) at += sh.part[w0];
+    const int r0 = w0 * run, r1 = min(n, r0 + run);
+    const int piece = (r1 - r0 + SP_THREADS - 1) / SP_THREADS * 32;   // and of that, a piece per warp
+    __syncthreads();
+    s = 0;
+    for (int i = r0 + warp * piece + lane; i < min(r1, r0 + (warp + 1) * piece); i += 32) s += kept_weight(i);
+    s = warp_add(s);
+    if (lane == 0) sh.part[warp] = s;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) at += sh.part[w];
+    if (goal < at || goal >= at + s) return;
+    for (int i0 = r0 + warp * piece; i0 < min(r1, r0 + (warp + 1) * piece); i0 += 32) {
+        const u64 w = i0 + lane < r1 ? kept_weight(i0 + lane) : 0;
+        u64 inc = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += y;
+        }
+        if (w && goal >= at + inc - w && goal < at + inc) a.tokens[row] = first + i0 + lane;
+        at += __shfl_sync(0xffffffffu, inc, 31);
+    }
+}
+
+// CTAs per row: as many as give the batch one CTA for every place on the GPU
+// (two per SM), so that a few rows are spread and many are not, but enough
+// that a slice fits. Measured at 32000 logits: TODO.
+static int sample_cluster(int rows, int vocab, int n_sm) {
+    int c = 1;
+    while (c < 8 && ((long long)rows * c * 2 <= 2 * n_sm || vocab > c * SP_SLICE)) c *= 2;
+    return c;
+}
+
+template <typename T>
+static cudaError_t launch_sample(const ptc_sample_args &a, int n_sm, cudaStream_t s) {
+    const int CL = sample_cluster(a.rows, a.vocab, n_sm), slice = (a.vocab + CL - 1) / CL;
+    const size_t smem = sizeof(SampleShared) + (size_t)slice * sizeof(T) + 32;
+    cudaError_t e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.rows * CL));
+    cfg.blockDim = dim3(SP_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CL;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_sample<T>, a, slice);
 }
 
 }  // namespace ptc
@@ -178,7 +608,7 @@ extern "C" int ptc_sample_tokens(const ptc_sample_args *p, void *stream) {
     if (!p) SERVE_REFUSE("no arguments");
     const ptc_sample_args a = *p;
     if (!ptc::dtype_ok(a.dtype)) SERVE_REFUSE("the logits' type is none of PTC_F32, PTC_F16, PTC_BF16");
-    if (a.rows < 0 || a.vocab < 1 || a.vocab > PTC_SAMPLE_MAX_VOCAB || a.stride < a.vocab)
+    if (a.rows < 0 || a.rows > (1 << 24) || a.vocab < 1 || a.vocab > PTC_SAMPLE_MAX_VOCAB || a.stride < a.vocab)
         SERVE_REFUSE("bad size (rows %d, vocab %d of at most %d, stride %lld)", a.rows, a.vocab, PTC_SAMPLE_MAX_VOCAB, a.stride);
     if (a.rows == 0) return 0;
     if (!a.logits || !a.u || !a.tokens) SERVE_REFUSE("a required pointer is NULL");
@@ -186,9 +616,10 @@ extern "C" int ptc_sample_tokens(const ptc_sample_args *p, void *stream) {
     cudaStream_t s = (cudaStream_t)stream;
     ptc::MemoryDevice on(a.tokens);
     SERVE_CUDA(on.error());
-    if (a.dtype == PTC_F32) ptc::k_sample<float><<<a.rows, ptc::SM_THREADS, 0, s>>>(a);
-    else if (a.dtype == PTC_F16) ptc::k_sample<__half><<<a.rows, ptc::SM_THREADS, 0, s>>>(a);
-    else ptc::k_sample<__nv_bfloat16><<<a.rows, ptc::SM_THREADS, 0, s>>>(a);
-    SERVE_CUDA(cudaGetLastError());
+    int n_sm = 0;
+    SERVE_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, on.device()));
+    if (a.dtype == PTC_F32) SERVE_CUDA(ptc::launch_sample<float>(a, n_sm, s));
+    else if (a.dtype == PTC_F16) SERVE_CUDA(ptc::launch_sample<__half>(a, n_sm, s));
+    else SERVE_CUDA(ptc::launch_sample<__nv_bfloat16>(a, n_sm, s));
     return 0;
 }
