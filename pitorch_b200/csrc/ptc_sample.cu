@@ -40,11 +40,12 @@ constexpr int SP_WARPS = SP_THREADS / 32;
 constexpr int SP_BINS = 4096;     // of the first histogram; the last one holds what has no weight
 constexpr int SP_BINS2 = 1024;    // of the second
 constexpr int SP_LIST = 1024;     // members that are ranked
-constexpr int SP_FEW = 256;       // ... without a second histogram
-constexpr int SP_PER = SP_BINS / SP_THREADS;
+constexpr int SP_FEW = 512;       // ... without a second histogram
 constexpr int SP_SLICE = 16384;   // logits of a CTA, while 8 of them hold the row
 constexpr float SP_RANGE = 44.f;  // weights below 2^-44 are zero
 typedef unsigned long long u64;
+// values that the CTAs of a row tell each other, a slot each
+enum { IN_BEST, IN_MASS, IN_COUNT, IN_OVER, IN_LIST, IN_BRACKET, IN_RANGE, IN_BEFORE, IN_MASS2, IN_SEG2, IN_OVER2, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
 constexpr double SP_ONE = 8796093022208.0;   // 2^43
 
 struct alignas(16) SampleShared {
@@ -58,11 +59,11 @@ struct alignas(16) SampleShared {
         } all;
     };
     u64 list[SP_LIST];   // this CTA's members
-    unsigned n_list[2];
     double table[32];    // 2^(j/32)
-    u64 part[SP_WARPS], box[6], step[2];   // sums of warps; values that the other CTAs read
-    u64 found;
-    int bin, above, in_bin, b_lo, b_hi, range_n;
+    u64 in[SP_SLOTS][8];   // what each CTA of the cluster pushed here, by value and rank
+    u64 part[SP_WARPS], part2[SP_WARPS];
+    u64 border[2], found, lo, hi;
+    unsigned n_list;
 };
 
 // A logit as the rules see it: NaN counts as -inf, and -0 as 0, so that equal
@@ -117,7 +118,7 @@ __device__ __forceinline__ u64 warp_top(u64 v) {
 }
 
 // The CTA's sum of v, in every thread.
-__device__ u64 block_add(u64 v, u64 *part) {
+__device__ __forceinline__ u64 block_add(u64 v, u64 *part) {
     v = warp_add(v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
@@ -128,23 +129,60 @@ __device__ u64 block_add(u64 v, u64 *part) {
     return t;
 }
 
-// The sum of `box` over the cluster (after a barrier of the cluster).
-__device__ u64 peers_sum(cg::cluster_group &cl, u64 *box) {
-    u64 t = 0;
-    for (unsigned q = 0; q < cl.num_blocks(); q++) t += *cl.map_shared_rank(box, q);
-    return t;
+// The sum of v over the threads before this one, and over all.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V *part, V &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    V inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+    }
+    __syncthreads();
+    if (lane == 31) part[warp] = inc;
+    __syncthreads();
+    V before = inc - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) {
+        if (w < warp) before += part[w];
+        total += part[w];
+    }
+    return before;
 }
 
-template <typename T>
+template <typename T, int CL>
 struct SampleRow {
     SampleShared &sh;
     cg::cluster_group &cl;
-    const T *x;     // this CTA's slice in shared memory
-    int n, first;   // its length and the index of its first logit
+    const T *x;       // this CTA's slice in shared memory
+    int n, first;     // its length and the index of its first logit
+    int rank;
     Weigh wt;
-    int turn;       // the slot of sh.step that the next sum takes: the other CTAs may still read the last one
+    int turn;         // which of the two IN_STEP slots the next sum takes: the other CTAs may still read the last one
 
     __device__ u64 key(float v, int i) const { return argmax_key(v, first + i); }
+
+    // v into every CTA's slot; there after the next barrier of the cluster.
+    // Stores overlap with the barrier, where loads after it would add a round
+    // trip each.
+    __device__ void push(int slot, u64 v) {
+        if (threadIdx.x < CL) *cl.map_shared_rank(&sh.in[slot][rank], threadIdx.x) = v;
+    }
+    __device__ u64 pushed(int slot) const {
+        u64 t = 0;
+#pragma unroll
+        for (int q = 0; q < CL; q++) t += sh.in[slot][q];
+        return t;
+    }
+    __device__ u64 pushed_before(int slot) const {
+        u64 t = 0;
+#pragma unroll
+        for (int q = 0; q < CL; q++)
+            if (q < rank) t += sh.in[slot][q];
+        return t;
+    }
 
     // Sum over the cluster of f(value, key), a barrier of the cluster in it.
     template <typename F>
@@ -154,12 +192,11 @@ struct SampleRow {
             const float v = logit(x[i]);
             s += f(v, key(v, i));
         }
-        s = block_add(s, sh.part);
-        u64 *slot = &sh.step[turn];
+        const int slot = IN_STEP + turn;
         turn ^= 1;
-        if (threadIdx.x == 0) *slot = s;
+        push(slot, block_add(s, sh.part));
         cl.sync();
-        return peers_sum(cl, slot);
+        return pushed(slot);
     }
 
     // The k-th largest key, by bisection.
@@ -184,54 +221,59 @@ struct SampleRow {
         return lo;
     }
 
-    // Collects the keys that `in` picks and, over the slice, the sum of `add`;
+    // Collects the keys that `in` picks and sums `add` over the rest of the row;
     // one barrier of the cluster. Every CTA then has all of them in sh.all.key
     // (their number is returned; more than SP_LIST: nothing to use). The two
-    // calls of a row use a list and a box each, as the other CTAs may still read
-    // the first when the second begins; the second's list takes the place of the
-    // first histogram, which everyone has read by then.
+    // calls of a row use a list each, as the other CTAs may still read the
+    // first when the second begins; the second's takes the place of the first
+    // histogram, which everyone has read by then.
     template <typename In, typename Add>
-    __device__ int collect(In in, Add add, u64 &total, int box, int second) {
+    __device__ int collect(In in, Add add, u64 &total, int slot, int second) {
         static_assert(sizeof(sh.hist) >= sizeof(sh.list), "the second list fits");
         u64 *list = second ? (u64 *)sh.hist : sh.list;
-        unsigned *count = &sh.n_list[second];
-        if (threadIdx.x == 0) *count = 0;
+        if (threadIdx.x == 0) sh.n_list = 0;
         __syncthreads();
         u64 s = 0;
+#pragma unroll 2
         for (int i = threadIdx.x; i < n; i += SP_THREADS) {
             const float v = logit(x[i]);
             const u64 e = key(v, i);
             const float f = wt.place(v);
             if (in(e, f)) {
-                const unsigned at = atomicAdd(count, 1u);
+                const unsigned at = atomicAdd(&sh.n_list, 1u);
                 if (at < SP_LIST) list[at] = e;
             } else {
                 s += add(v, e, f);
             }
         }
         s = block_add(s, sh.part);
-        if (threadIdx.x == 0) sh.box[box] = s;
+        push(slot, s);
+        push(slot + 1, min(sh.n_list, (unsigned)SP_LIST + 1));
         cl.sync();
-        total = peers_sum(cl, &sh.box[box]);
-        int at = 0;
-        for (unsigned q = 0; q < cl.num_blocks(); q++) {
-            const int c = (int)min(*cl.map_shared_rank(count, q), (unsigned)SP_LIST + 1);
-            const u64 *from = cl.map_shared_rank(list, q);
-            if (at + c <= SP_LIST)
-                for (int i = threadIdx.x; i < c; i += SP_THREADS) sh.all.key[at + i] = from[i];
-            at = min(at + c, SP_LIST + 1);
+        total = pushed(slot);
+        const int m = (int)pushed(slot + 1);
+        if (m <= SP_LIST) {
+            for (int i = threadIdx.x; i < m; i += SP_THREADS) {
+                int q = 0, at = i;   // member i is the at-th of CTA q
+#pragma unroll
+                for (int k = 0; k < CL - 1; k++) {
+                    const int c = (int)sh.in[slot + 1][k];
+                    if (q == k && at >= c) at -= c, q++;
+                }
+                sh.all.key[i] = cl.map_shared_rank(list, q)[at];
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        return at;
+        return m;
     }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int slice) {
+template <typename T, int CL>
+__global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int slice) {
     extern __shared__ __align__(16) char sp_smem[];
     SampleShared &sh = *(SampleShared *)sp_smem;
     cg::cluster_group cl = cg::this_cluster();
-    const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank(), row = blockIdx.x / CL;
+    const int rank = (int)cl.block_rank(), row = blockIdx.x / CL;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = min(a.vocab, rank * slice), n = min(slice, a.vocab - first);
 
@@ -244,6 +286,7 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
     {
         float top = -INFINITY;
         int at = -1;
+#pragma unroll 4
         for (int v = tid; v * N < n + shift; v += SP_THREADS) {
             const int i0 = v * N - shift;
             if (i0 >= 0 && i0 + N <= n) {
@@ -265,36 +308,38 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
         }
         if (at >= 0) best = argmax_key(top, first + at);
     }
-    for (int i = tid; i < SP_BINS; i += SP_THREADS) sh.hist[i] = 0;
+    for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid < 32) sh.table[tid] = exp2((double)tid / 32.0);
+    const float temp = a.temperature ? a.temperature[row] : 1.0f;
+    const int want_k = a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+    SampleRow<T, CL> R = {sh, cl, x, n, first, rank, {}, 0};
     best = warp_top(best);
     if (lane == 0) sh.part[warp] = best;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 0; w < SP_WARPS; w++) best = max(best, sh.part[w]);
-        sh.box[0] = best;
-    }
+    if (tid == 0) sh.lo = sh.hi = sh.border[1] = ~0ull;
+    cl.sync();   // every CTA of the cluster runs: its shared memory may be written
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) best = max(best, sh.part[w]);
+    R.push(IN_BEST, best);
     cl.sync();
-    best = 0;
-    for (int q = 0; q < CL; q++) best = max(best, *cl.map_shared_rank(&sh.box[0], q));
+#pragma unroll
+    for (int q = 0; q < CL; q++) best = max(best, sh.in[IN_BEST][q]);
 
-    const float temp = a.temperature ? a.temperature[row] : 1.0f, top = key_value(best);
+    const float top = key_value(best);
     if (top == -INFINITY || !(temp > 0.0f)) {
         if (tid == 0 && rank == 0) a.tokens[row] = top == -INFINITY ? -1 : argmax_key_index(best);
-        cl.sync();   // nobody reads a CTA's shared memory after it has left
         return;
     }
     const double c = 1.4426950408889634 / (double)temp;
     const Weigh wt = {top, (float)((SP_BINS - 1) / SP_RANGE * c), c, (double)top * c, sh.table};
-    SampleRow<T> R = {sh, cl, x, n, first, wt, 0};
-    const int want_k = a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
+    R.wt = wt;
     const bool by_k = want_k > 0 && want_k < a.vocab, by_p = p < 1.0f;
     u64 floor_key = 0;   // tokens with a key at or above it are kept
 
     if (by_k || by_p) {
         // counts of the bins; with top_p alone, the mass of the row
         u64 mass = 0;
+#pragma unroll 4
         for (int i = tid; i < n; i += SP_THREADS) {
             const float v = logit(x[i]);
             const int b = Weigh::bin(wt.place(v));
@@ -303,60 +348,50 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
                 if (!by_k) mass += wt.weight(v);
             }
         }
-        mass = block_add(mass, sh.part);
-        if (tid == 0) {
-            sh.box[1] = mass;
-            sh.bin = SP_BINS - 1;
-        }
+        R.push(IN_MASS, block_add(mass, sh.part));
         cl.sync();
-        u64 total = peers_sum(cl, &sh.box[1]);
-        int cnt[SP_PER], mine = 0;
+        u64 total = R.pushed(IN_MASS);
+        // each CTA adds up its share of the bins, PER to a thread
+        constexpr int PER = SP_BINS / CL / SP_THREADS;
+        const int bin0 = (rank * SP_THREADS + tid) * PER;
+        int cnt[PER], mine = 0;
 #pragma unroll
-        for (int i = 0; i < SP_PER; i++) cnt[i] = 0;
+        for (int i = 0; i < PER; i++) cnt[i] = 0;
+#pragma unroll
         for (int q = 0; q < CL; q++) {
-            const uint4 *h = (const uint4 *)(cl.map_shared_rank(sh.hist, q) + tid * SP_PER);
+            const unsigned *h = cl.map_shared_rank(sh.hist, (rank + q) % CL) + bin0;   // not all from the same CTA at once
 #pragma unroll
-            for (int i = 0; i < SP_PER / 4; i++) {
-                const uint4 u = h[i];
-                cnt[4 * i] += u.x;
-                cnt[4 * i + 1] += u.y;
-                cnt[4 * i + 2] += u.z;
-                cnt[4 * i + 3] += u.w;
-            }
+            for (int i = 0; i < PER; i++) cnt[i] += h[i];
         }
 #pragma unroll
-        for (int i = 0; i < SP_PER; i++) mine += cnt[i];
+        for (int i = 0; i < PER; i++) mine += cnt[i];
         if (by_k) {
-            int inc = mine;
+            int own;
+            int before = block_scan(mine, (int *)sh.part, own);
+            R.push(IN_COUNT, own);
+            cl.sync();
+            before += (int)R.pushed_before(IN_COUNT);
+            if ((int)R.pushed(IN_COUNT) >= want_k) {   // else all that has weight is among the k largest
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += y;
-            }
-            __syncthreads();
-            if (lane == 31) sh.part[warp] = inc;
-            __syncthreads();
-            int before = inc - mine;
-            for (int w = 0; w < warp; w++) before += (int)sh.part[w];
-#pragma unroll
-            for (int i = 0; i < SP_PER; i++) {   // the bin in which the count reaches k
-                if (before < want_k && before + cnt[i] >= want_k) sh.bin = tid * SP_PER + i, sh.above = before, sh.in_bin = cnt[i];
-                before += cnt[i];
-            }
-            __syncthreads();
-            const int bk = sh.bin;
-            if (bk < SP_BINS - 1) {   // else all that has weight is among the k largest
-                const int rest = want_k - sh.above;   // of the bin's members
+                for (int i = 0; i < PER; i++) {   // the bin in which the count reaches k, to every CTA
+                    if (before < want_k && before + cnt[i] >= want_k)
+                        for (int q = 0; q < CL; q++)
+                            *cl.map_shared_rank(&sh.border[0], q) = (u64)(bin0 + i) << 40 | (u64)before << 20 | (u64)cnt[i];
+                    before += cnt[i];
+                }
+                cl.sync();
+                const int bk = (int)(sh.border[0] >> 40), in_bin = (int)(sh.border[0] & 0xfffff);
+                const int rest = want_k - (int)(sh.border[0] >> 20 & 0xfffff);   // of the bin's members
                 u64 over = 0;
-                const int m = sh.in_bin <= SP_LIST ? R.collect([&](u64, float f) { return Weigh::bin(f) == bk; },
-                                                               [&](float v, u64, float f) { return by_p && Weigh::bin(f) < bk ? wt.weight(v) : 0; }, over, 2, 0)
-                                                   : SP_LIST + 1;
-                if (m <= SP_LIST) {
+                if (in_bin <= SP_LIST) {
+                    const int m = R.collect([&](u64, float f) { return Weigh::bin(f) == bk; },
+                                            [&](float v, u64, float f) { return by_p && Weigh::bin(f) < bk ? wt.weight(v) : 0; }, over, IN_OVER, 0);
                     for (int i = tid; i < m; i += SP_THREADS) {
                         const u64 e = sh.all.key[i];
-                        int rank_ = 0;
-                        for (int j = 0; j < m; j++) rank_ += sh.all.key[j] > e;
-                        if (rank_ == rest - 1) sh.found = e;
+                        int above = 0;
+#pragma unroll 4
+                        for (int j = 0; j < m; j++) above += sh.all.key[j] > e;
+                        if (above == rest - 1) sh.found = e;
                     }
                     __syncthreads();
                     floor_key = sh.found;
@@ -372,10 +407,9 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
                 }
                 // the counts that are left for top_p
 #pragma unroll
-                for (int i = 0; i < SP_PER; i++) {
-                    const int b = tid * SP_PER + i;
-                    if (b == bk) cnt[i] = rest;
-                    if (b > bk) cnt[i] = 0;
+                for (int i = 0; i < PER; i++) {
+                    if (bin0 + i == bk) cnt[i] = rest;
+                    if (bin0 + i > bk) cnt[i] = 0;
                 }
             } else if (by_p) {
                 total = R.sum([&](float v, u64) { return wt.weight(v); });
@@ -387,53 +421,63 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
             if (want > 0) {
                 // bracket from the counts: bins whose mass can hold the border
                 const float q = SP_RANGE / (SP_BINS - 1), goal = (float)(want / SP_ONE);
-                float low = 0.f, high = 0.f;
+                float low = 0.f, high = 0.f, lows[PER], highs[PER];
+                mine = 0;
 #pragma unroll
-                for (int i = 0; i < SP_PER; i++) {
-                    const float b = (float)(tid * SP_PER + i);
-                    low += cnt[i] * exp2f(-(b + 1.01f) * q);
-                    high += cnt[i] * exp2f(-(b - 0.01f) * q);
+                for (int i = 0; i < PER; i++) {
+                    const float b = (float)(bin0 + i);
+                    low += lows[i] = cnt[i] * exp2f(-(b + 1.01f) * q);
+                    high += highs[i] = cnt[i] * exp2f(-(b - 0.01f) * q);
+                    mine += cnt[i];
                 }
-                float il = low, ih = high;
+                float own_l, own_h;
+                int own;
+                float bl = block_scan(low, (float *)sh.part, own_l), bh = block_scan(high, (float *)sh.part2, own_h);
+                int before = block_scan(mine, (int *)sh.part, own);
+                R.push(IN_BRACKET, (u64)__float_as_uint(own_l) << 32 | __float_as_uint(own_h));
+                R.push(IN_BEFORE, own);
+                cl.sync();
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const float y = __shfl_up_sync(0xffffffffu, il, o), z = __shfl_up_sync(0xffffffffu, ih, o);
-                    if (lane >= o) il += y, ih += z;
-                }
-                float2 *fp = (float2 *)sh.part;
-                __syncthreads();
-                if (tid == 0) sh.b_lo = SP_BINS - 2, sh.b_hi = SP_BINS - 2, sh.range_n = 0;
-                if (lane == 31) fp[warp] = make_float2(il, ih);
-                __syncthreads();
-                float bl = il - low, bh = ih - high;
-                for (int w = 0; w < warp; w++) bl += fp[w].x, bh += fp[w].y;
+                for (int r = 0; r < CL; r++)
+                    if (r < rank) bl += __uint_as_float((unsigned)(sh.in[IN_BRACKET][r] >> 32)), bh += __uint_as_float((unsigned)sh.in[IN_BRACKET][r]);
+                before += (int)R.pushed_before(IN_BEFORE);
+                // first bin that may reach the goal, with the count before it; first that must, with the count through it
+                u64 lo = ~0ull, hi = ~0ull;
 #pragma unroll
-                for (int i = 0; i < SP_PER; i++) {
-                    const int b = tid * SP_PER + i;
-                    bl += cnt[i] * exp2f(-((float)b + 1.01f) * q);
-                    bh += cnt[i] * exp2f(-((float)b - 0.01f) * q);
-                    if (bh * 1.0001f >= goal) atomicMin(&sh.b_lo, b);
-                    if (bl * 0.9999f >= goal) atomicMin(&sh.b_hi, b);
+                for (int i = 0; i < PER; i++) {
+                    bl += lows[i];
+                    bh += highs[i];
+                    if (lo == ~0ull && bh * 1.0001f >= goal) lo = (u64)(bin0 + i) << 20 | (u64)before;
+                    before += cnt[i];
+                    if (hi == ~0ull && bl * 0.9999f >= goal) hi = (u64)(bin0 + i) << 20 | (u64)before;
                 }
+                const unsigned los = __ballot_sync(0xffffffffu, lo != ~0ull), his = __ballot_sync(0xffffffffu, hi != ~0ull);
+                if (los && lane == __ffs(los) - 1) atomicMin(&sh.lo, lo);
+                if (his && lane == __ffs(his) - 1) atomicMin(&sh.hi, hi);
                 __syncthreads();
-                const int b_lo = sh.b_lo, b_hi = max(sh.b_hi, b_lo);
-                int in_range = 0;
+                R.push(IN_RANGE, (sh.lo & 0xffffffffull) << 32 | (sh.hi & 0xffffffffull));
+                cl.sync();
+                unsigned range_lo = ~0u, range_hi = ~0u;
 #pragma unroll
-                for (int i = 0; i < SP_PER; i++) {
-                    const int b = tid * SP_PER + i;
-                    if (b >= b_lo && b <= b_hi) in_range += cnt[i];
+                for (int r = 0; r < CL; r++) {
+                    range_lo = min(range_lo, (unsigned)(sh.in[IN_RANGE][r] >> 32));
+                    range_hi = min(range_hi, (unsigned)sh.in[IN_RANGE][r]);
                 }
-                if (in_range) atomicAdd(&sh.range_n, in_range);
-                __syncthreads();
+                const int all = (int)R.pushed(IN_BEFORE);
+                if (range_hi == ~0u) range_hi = (unsigned)(SP_BINS - 2) << 20 | (unsigned)all;
+                if (range_lo == ~0u) range_lo = (unsigned)(SP_BINS - 2) << 20 | (unsigned)all;
+                const int b_lo = (int)(range_lo >> 20), b_hi = max(b_lo, (int)(range_hi >> 20));
+                const int in_range = (int)(range_hi & 0xfffff) - (int)(range_lo & 0xfffff);
                 u64 over = 0;
                 int g_lo = 0, g_hi = SP_BINS2;   // the second histogram's bins that are collected
                 const float g_scale = (float)SP_BINS2 / (float)(b_hi - b_lo + 1);
                 auto sub = [&](float f) { return min(SP_BINS2 - 1, (int)((f - (float)b_lo) * g_scale)); };
                 auto inside = [&](u64 e, float f) { return e >= floor_key && Weigh::bin(f) >= b_lo && Weigh::bin(f) <= b_hi; };
-                if (sh.range_n > SP_FEW) {
+                if (in_range > SP_FEW) {
                     for (int i = tid; i < 3 * SP_BINS2; i += SP_THREADS) ((unsigned *)sh.mass)[i] = 0;
                     __syncthreads();
                     u64 s = 0;
+#pragma unroll 2
                     for (int i = tid; i < n; i += SP_THREADS) {
                         const float v = logit(x[i]), f = wt.place(v);
                         const u64 e = R.key(v, i);
@@ -448,48 +492,46 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
                             atomicAdd(&sh.mass[2][g], (unsigned)(w >> 30));
                         }
                     }
-                    s = block_add(s, sh.part);
-                    if (tid == 0) sh.box[3] = s, sh.bin = -1;
+                    R.push(IN_MASS2, block_add(s, sh.part));
                     cl.sync();
-                    const u64 before = peers_sum(cl, &sh.box[3]);
-                    constexpr int PER = SP_BINS2 / SP_THREADS;
-                    u64 m[PER], sum = 0;
+                    const u64 sure = R.pushed(IN_MASS2);
+                    constexpr int SEG2 = SP_BINS2 / CL, PER2 = SEG2 > SP_THREADS ? SEG2 / SP_THREADS : 1;
+                    const int g0 = rank * SEG2 + tid * PER2;
+                    u64 m[PER2], sum = 0, own_m;
 #pragma unroll
-                    for (int i = 0; i < PER; i++) m[i] = 0;
-                    for (int r = 0; r < CL; r++) {
-                        const unsigned *h = cl.map_shared_rank((unsigned *)sh.mass, r) + tid * PER;
+                    for (int i = 0; i < PER2; i++) m[i] = 0;
+                    if (tid * PER2 < SEG2) {
 #pragma unroll
-                        for (int i = 0; i < PER; i++) m[i] += h[i] + ((u64)h[SP_BINS2 + i] << 15) + ((u64)h[2 * SP_BINS2 + i] << 30);
+                        for (int r = 0; r < CL; r++) {
+                            const unsigned *h = cl.map_shared_rank((unsigned *)sh.mass, (rank + r) % CL) + g0;
+#pragma unroll
+                            for (int i = 0; i < PER2; i++) m[i] += h[i] + ((u64)h[SP_BINS2 + i] << 15) + ((u64)h[2 * SP_BINS2 + i] << 30);
+                        }
                     }
 #pragma unroll
-                    for (int i = 0; i < PER; i++) sum += m[i];
-                    u64 inc = sum;
+                    for (int i = 0; i < PER2; i++) sum += m[i];
+                    u64 at = block_scan(sum, sh.part, own_m);
+                    R.push(IN_SEG2, own_m);
+                    cl.sync();
+                    at += sure + R.pushed_before(IN_SEG2);
 #pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-                        if (lane >= o) inc += y;
-                    }
-                    __syncthreads();
-                    if (lane == 31) sh.part[warp] = inc;
-                    __syncthreads();
-                    u64 at = before + inc - sum;
-                    for (int w = 0; w < warp; w++) at += sh.part[w];
-#pragma unroll
-                    for (int i = 0; i < PER; i++) {   // the bin in which the mass reaches the goal
-                        if ((double)at < want && (double)(at + m[i]) >= want) sh.bin = tid * PER + i;
+                    for (int i = 0; i < PER2; i++) {   // the bin in which the mass reaches the goal, to every CTA
+                        if ((double)at < want && (double)(at + m[i]) >= want)
+                            for (int r = 0; r < CL; r++) *cl.map_shared_rank(&sh.border[1], r) = (u64)(g0 + i);
                         at += m[i];
                     }
-                    __syncthreads();
-                    g_lo = sh.bin;
+                    cl.sync();
+                    g_lo = sh.border[1] == ~0ull ? -1 : (int)sh.border[1];
                     g_hi = g_lo + 1;
                 }
                 // rank what is left by mass: e is kept while less than the goal is above it
-                const int m = g_lo < 0 ? SP_LIST + 1
-                                       : R.collect([&](u64 e, float f) { return inside(e, f) && sub(f) >= g_lo && sub(f) < g_hi; },
-                                                   [&](float v, u64 e, float f) {
-                                                       const int b = Weigh::bin(f);
-                                                       return e >= floor_key && (b < b_lo || (b <= b_hi && sub(f) < g_lo)) ? wt.weight(v) : 0;
-                                                   }, over, 4, by_k);
+                int m = SP_LIST + 1;
+                if (g_lo >= 0)
+                    m = R.collect([&](u64 e, float f) { return inside(e, f) && sub(f) >= g_lo && sub(f) < g_hi; },
+                                  [&](float v, u64 e, float f) {
+                                      const int b = Weigh::bin(f);
+                                      return e >= floor_key && (b < b_lo || (b <= b_hi && sub(f) < g_lo)) ? wt.weight(v) : 0;
+                                  }, over, IN_OVER2, by_k);
                 bool done = false;
                 if (m <= SP_LIST) {
                     for (int i = tid; i < m; i += SP_THREADS) sh.all.w[i] = wt.weight(key_value(sh.all.key[i]));
@@ -498,8 +540,8 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
                     for (int i = tid; i < m; i += SP_THREADS) {
                         const u64 e = sh.all.key[i];
                         u64 above = over;
-                        for (int j = 0; j < m; j++)
-                            if (sh.all.key[j] > e) above += sh.all.w[j];
+#pragma unroll 4
+                        for (int j = 0; j < m; j++) above += sh.all.key[j] > e ? sh.all.w[j] : 0;
                         if ((double)above < want) atomicMin(&sh.found, e);
                     }
                     __syncthreads();
@@ -513,7 +555,6 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
     }
 
     // The kept weights in index order: a warp has a run of the slice.
-    const float mp = a.min_p ? a.min_p[row] : 0.0f;
     const double least = (mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE;
     auto kept_weight = [&](int i) -> u64 {
         const float v = logit(x[i]);
@@ -523,27 +564,21 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
     };
     const int run = (n + SP_THREADS - 1) / SP_THREADS * 32;
     u64 s = 0;
-    for (int i = warp * run + lane; i < min(n, (warp + 1) * run); i += 32) s += kept_weight(i);
+    const int end = min(n, (warp + 1) * run);
+#pragma unroll 4
+    for (int i = warp * run + lane; i < end; i += 32) s += kept_weight(i);
     s = warp_add(s);
     __syncthreads();
     if (lane == 0) sh.part[warp] = s;
     __syncthreads();
-    if (tid == 0) {
-        u64 t = 0;
-        for (int w = 0; w < SP_WARPS; w++) t += sh.part[w];
-        sh.box[5] = t;
-    }
-    cl.sync();
-    u64 before = 0, total = 0, own = 0;
-    for (int q = 0; q < CL; q++) {
-        const u64 t = *cl.map_shared_rank(&sh.box[5], q);
-        if (q < rank) before += t;
-        if (q == rank) own = t;
-        total += t;
-    }
-    cl.sync();   // the others may leave
-    const double u = (double)a.u[row] * (double)total;
-    u64 goal = u > 0 ? (u < (double)total ? (u64)u : total - 1) : 0;
+    u64 own = 0;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; w++) own += sh.part[w];
+    R.push(IN_KEPT, own);
+    cl.sync();   // the last access to another CTA is before it, so each may leave from here on
+    const u64 before = R.pushed_before(IN_KEPT), total = R.pushed(IN_KEPT);
+    const double ut = (double)u * (double)total;
+    u64 goal = ut > 0 ? (ut < (double)total ? (u64)ut : total - 1) : 0;
     if (goal >= total) goal = total - 1;
     if (goal < before || goal >= before + own) return;
     goal -= before;
@@ -552,13 +587,12 @@ __global__ void __launch_bounds__(SP_THREADS) k_sample(ptc_sample_args a, int sl
     for (; w0 < SP_WARPS - 1 && at + sh.part[w0] <= goal; w0++) at += sh.part[w0];
     const int r0 = w0 * run, r1 = min(n, r0 + run);
     const int piece = (r1 - r0 + SP_THREADS - 1) / SP_THREADS * 32;   // and of that, a piece per warp
-    __syncthreads();
     s = 0;
     for (int i = r0 + warp * piece + lane; i < min(r1, r0 + (warp + 1) * piece); i += 32) s += kept_weight(i);
     s = warp_add(s);
-    if (lane == 0) sh.part[warp] = s;
+    if (lane == 0) sh.part2[warp] = s;
     __syncthreads();
-    for (int w = 0; w < warp; w++) at += sh.part[w];
+    for (int w = 0; w < warp; w++) at += sh.part2[w];
     if (goal < at || goal >= at + s) return;
     for (int i0 = r0 + warp * piece; i0 < min(r1, r0 + (warp + 1) * piece); i0 += 32) {
         const u64 w = i0 + lane < r1 ? kept_weight(i0 + lane) : 0;
@@ -582,11 +616,11 @@ static int sample_cluster(int rows, int vocab, int n_sm) {
     return c;
 }
 
-template <typename T>
-static cudaError_t launch_sample(const ptc_sample_args &a, int n_sm, cudaStream_t s) {
-    const int CL = sample_cluster(a.rows, a.vocab, n_sm), slice = (a.vocab + CL - 1) / CL;
+template <typename T, int CL>
+static cudaError_t launch_sample_cl(const ptc_sample_args &a, cudaStream_t s) {
+    const int slice = (a.vocab + CL - 1) / CL;
     const size_t smem = sizeof(SampleShared) + (size_t)slice * sizeof(T) + 32;
-    cudaError_t e = cudaFuncSetAttribute(k_sample<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(k_sample<T, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * CL));
@@ -599,7 +633,17 @@ static cudaError_t launch_sample(const ptc_sample_args &a, int n_sm, cudaStream_
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_sample<T>, a, slice);
+    return cudaLaunchKernelEx(&cfg, k_sample<T, CL>, a, slice);
+}
+
+template <typename T>
+static cudaError_t launch_sample(const ptc_sample_args &a, int n_sm, cudaStream_t s) {
+    switch (sample_cluster(a.rows, a.vocab, n_sm)) {
+    case 1: return launch_sample_cl<T, 1>(a, s);
+    case 2: return launch_sample_cl<T, 2>(a, s);
+    case 4: return launch_sample_cl<T, 4>(a, s);
+    default: return launch_sample_cl<T, 8>(a, s);
+    }
 }
 
 }  // namespace ptc
