@@ -1,24 +1,29 @@
 // ptc_sample.cu -- sampling of the next tokens on the GPU (include/ptc_serve.h).
 //
 // A cluster of 1 to 8 CTAs per row; each holds its slice of the logits in
-// shared memory, so the row is read from memory once. Nothing is sorted. The
-// kept tokens are those whose (value, lowest index first) key is at or above
-// one threshold, which is found by counting:
+// shared memory, so the row is read from memory once. Nothing is sorted: the
+// kept tokens are those at or above one threshold in the order (value, lowest
+// index first), which is found by counting.
 //
-//  1. the maximum;
-//  2. a histogram of the logits by their distance from it (4096 bins of equal
-//     width down to where a weight is zero), exchanged through distributed
-//     shared memory. The bin that holds the k-th largest is collected and its
-//     few members ranked: the threshold of top_k;
-//  3. top_p: a bin's mass lies between its count times its lowest and highest
+// Few kept (top_k up to 512): each thread's maximum is known from the load,
+// and the bin in which k of these maxima lie is low enough to hold the k
+// largest of all, and little more. One comparison per logit collects them (a
+// few hundred) in one CTA, which ranks them against each other for all the
+// rules.
+//
+// Otherwise:
+//  1. a histogram of the logits by their distance from the maximum (4096 bins
+//     of equal width down to where a weight is zero), added up through
+//     distributed shared memory. The bin that holds the k-th largest is
+//     collected and its members ranked: the threshold of top_k;
+//  2. top_p: a bin's mass lies between its count times its lowest and highest
 //     weight, 0.8% apart, so the counts alone bracket the bins in which the
 //     mass can reach top_p times the total. The mass before the bracket is
-//     summed exactly; inside it, a second histogram of exact masses (1024
-//     bins) or, where there are few members, their ranking finds the last one
-//     kept;
-//  4. min_p is a comparison with the weight, and the token is found from the
+//     summed exactly; inside it, the ranking of its members, after a second
+//     histogram of exact masses (1024 bins) where they are many, finds the
+//     last one kept;
+//  3. min_p is a comparison with the weight, and the token is found from the
 //     kept sums of the CTAs, of their warps and of one warp's elements.
-//
 // Where a bin has too many members to be ranked (equal logits by the
 // thousand), the threshold is bisected instead.
 //
@@ -29,6 +34,7 @@
 // running sum of 10^5 weights has to be exact to far better than the weight
 // of one token, which 32-bit exponentials do not give.
 #include <cooperative_groups.h>
+#include <limits.h>
 
 #include "ptc_serve.cuh"
 
@@ -45,7 +51,7 @@ constexpr int SP_SLICE = 16384;   // logits of a CTA, while 8 of them hold the r
 constexpr float SP_RANGE = 44.f;  // weights below 2^-44 are zero
 typedef unsigned long long u64;
 // values that the CTAs of a row tell each other, a slot each
-enum { IN_BEST, IN_MASS, IN_COUNT, IN_OVER, IN_LIST, IN_BRACKET, IN_RANGE, IN_BEFORE, IN_MASS2, IN_SEG2, IN_OVER2, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
+enum { IN_BEST, IN_FEW, IN_MASS, IN_COUNT, IN_OVER, IN_LIST, IN_BRACKET, IN_RANGE, IN_BEFORE, IN_MASS2, IN_SEG2, IN_OVER2, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
 constexpr double SP_ONE = 8796093022208.0;   // 2^43
 
 struct alignas(16) SampleShared {
@@ -63,19 +69,22 @@ struct alignas(16) SampleShared {
     u64 in[SP_SLOTS][8];   // what each CTA of the cluster pushed here, by value and rank
     u64 part[SP_WARPS], part2[SP_WARPS];
     u64 border[2], found, lo, hi;
-    unsigned n_list;
+    unsigned n_list, n_few;
 };
 
-// A logit as the rules see it: NaN counts as -inf, and -0 as 0, so that equal
-// values have equal keys.
-template <typename T>
-__device__ __forceinline__ float logit(T v) {
-    const float x = Elem<T>::up(v);
-    return x != x ? -INFINITY : x + 0.0f;
-}
 __device__ __forceinline__ float key_value(u64 key) {
     const uint32_t k = (uint32_t)(key >> 32);
     return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+}
+
+// The order of the rules: larger value first, then lower index; -0 equals 0.
+__device__ __forceinline__ u64 order_key(float v, int i) { return argmax_key(v + 0.0f, i); }
+
+// A float that is no infinity as a double, by its bits (the conversion
+// instruction has a quarter of the rate); subnormals become 0.
+__device__ __forceinline__ double widen(float x) {
+    const uint32_t u = __float_as_uint(x), m = u & 0x7fffffffu;
+    return m < 0x00800000u ? 0.0 : __hiloint2double((int)((u & 0x80000000u) | ((m >> 3) + 0x38000000u)), (int)(u << 29));
 }
 
 // How a row's logits become bins and weights.
@@ -84,15 +93,17 @@ struct Weigh {
     double c, topc;     // log2(e) / temperature, and times the maximum
     const double *table;
 
-    __device__ float place(float x) const { return x == top ? 0.f : (top - x) * scale; }
-    __device__ static int bin(float f) { return f < (float)(SP_BINS - 1) ? (int)f : SP_BINS - 1; }
+    // Distance from the maximum in bins; NaN for an infinite maximum itself.
+    __device__ float place(float x) const { return (top - x) * scale; }
+    __device__ static bool heavy(float f) { return !(f >= (float)(SP_BINS - 1)); }   // has weight
+    __device__ static int bin(float f) { return heavy(f) ? (int)f : SP_BINS - 1; }
     // 2^y for y = (x - top) log2(e) / temperature: y = n/32 + r, 2^(n/32) from
     // the table and the exponent, 2^r by its series (ln 2)^i / i!
     __device__ u64 weight(float x) const {
+        if (!heavy(place(x))) return 0;
         if (x == top) return 1ull << 43;
-        if (!(place(x) < (float)(SP_BINS - 1))) return 0;
         const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the rounded integer
-        const double y = fma((double)x, c, -topc), t = fma(y, 32.0, magic);
+        const double y = fma(widen(x), c, -topc), t = fma(y, 32.0, magic);
         const int n = __double2loint(t);
         const double r = fma(t - magic, -1.0 / 32.0, y);
         double p = 1.3333558146428443e-3;
@@ -104,6 +115,14 @@ struct Weigh {
         p = __hiloint2double(__double2hiint(p) + (((n >> 5) + 43) << 20), __double2loint(p));
         return (u64)__double_as_longlong(p + 4503599627370496.0) & ((1ull << 52) - 1);
     }
+};
+
+// The threshold: kept are the logits above `v`, and those equal to it up to index `i`.
+struct Floor {
+    float v;
+    int i;
+    __device__ bool keeps(float x, int at) const { return x > v || (x == v && at <= i); }
+    __device__ static Floor of(u64 key) { return {key_value(key), argmax_key_index(key)}; }
 };
 
 __device__ __forceinline__ u64 warp_add(u64 v) {
@@ -154,15 +173,25 @@ __device__ __forceinline__ V block_scan(V v, V *part, V &total) {
 
 template <typename T, int CL>
 struct SampleRow {
+    static constexpr int N = Vec16<T>::N;
     SampleShared &sh;
     cg::cluster_group &cl;
-    const T *x;       // this CTA's slice in shared memory
-    int n, first;     // its length and the index of its first logit
+    const Vec16<T> *x;   // this CTA's slice in shared memory, -inf before and behind it
+    int vecs, first;     // its vectors, and the index of the first one's first element
     int rank;
     Weigh wt;
     int turn;         // which of the two IN_STEP slots the next sum takes: the other CTAs may still read the last one
 
-    __device__ u64 key(float v, int i) const { return argmax_key(v, first + i); }
+    // f(value, index) for this thread's share of the slice
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+        for (int v = threadIdx.x; v < vecs; v += SP_THREADS) {
+            const Vec16<T> e = x[v];
+#pragma unroll
+            for (int k = 0; k < N; k++) f(Elem<T>::up(e.e[k]), first + v * N + k);
+        }
+    }
 
     // v into every CTA's slot; there after the next barrier of the cluster.
     // Stores overlap with the barrier, where loads after it would add a round
@@ -184,14 +213,24 @@ struct SampleRow {
         return t;
     }
 
+    // The counts of PER bins from bin0 on, over the cluster.
+    template <int PER>
+    __device__ void gather(unsigned *hist, int bin0, int (&cnt)[PER]) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) cnt[i] = 0;
+#pragma unroll
+        for (int q = 0; q < CL; q++) {
+            const unsigned *h = cl.map_shared_rank(hist, (rank + q) % CL) + bin0;   // not all from the same CTA at once
+#pragma unroll
+            for (int i = 0; i < PER; i++) cnt[i] += h[i];
+        }
+    }
+
     // Sum over the cluster of f(value, key), a barrier of the cluster in it.
     template <typename F>
     __device__ u64 sum(F f) {
         u64 s = 0;
-        for (int i = threadIdx.x; i < n; i += SP_THREADS) {
-            const float v = logit(x[i]);
-            s += f(v, key(v, i));
-        }
+        each([&](float v, int i) { s += f(v, order_key(v, i)); });
         const int slot = IN_STEP + turn;
         turn ^= 1;
         push(slot, block_add(s, sh.part));
@@ -221,7 +260,7 @@ struct SampleRow {
         return lo;
     }
 
-    // Collects the keys that `in` picks and sums `add` over the rest of the row;
+    // Collects the keys of what `in` picks and sums `add` over the rest of the row;
     // one barrier of the cluster. Every CTA then has all of them in sh.all.key
     // (their number is returned; more than SP_LIST: nothing to use). The two
     // calls of a row use a list each, as the other CTAs may still read the
@@ -234,18 +273,15 @@ struct SampleRow {
         if (threadIdx.x == 0) sh.n_list = 0;
         __syncthreads();
         u64 s = 0;
-#pragma unroll 2
-        for (int i = threadIdx.x; i < n; i += SP_THREADS) {
-            const float v = logit(x[i]);
-            const u64 e = key(v, i);
+        each([&](float v, int i) {
             const float f = wt.place(v);
-            if (in(e, f)) {
+            if (in(v, i, f)) {
                 const unsigned at = atomicAdd(&sh.n_list, 1u);
-                if (at < SP_LIST) list[at] = e;
+                if (at < SP_LIST) list[at] = order_key(v, i);
             } else {
-                s += add(v, e, f);
+                s += add(v, i, f);
             }
-        }
+        });
         s = block_add(s, sh.part);
         push(slot, s);
         push(slot + 1, min(sh.n_list, (unsigned)SP_LIST + 1));
@@ -268,6 +304,64 @@ struct SampleRow {
     }
 };
 
+// The running sum that the token has to exceed.
+__device__ __forceinline__ u64 sample_goal(float u, u64 total) {
+    const double t = (double)u * (double)total;
+    const u64 goal = t > 0 ? (t < (double)total ? (u64)t : total - 1) : 0;
+    return min(goal, total - 1);
+}
+
+// All the rules on m collected logits, among them the k largest: each is
+// ranked against the others, by one CTA.
+__device__ void few_tokens(const ptc_sample_args &a, SampleShared &sh, const Weigh &wt, int row, int m, int k, float p, u64 least, float u) {
+    constexpr int EACH = SP_LIST / SP_THREADS;
+    const int tid = threadIdx.x;
+    u64 key[EACH], w[EACH], before[EACH], kept = 0;
+    int above[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int i = tid + e * SP_THREADS;
+        key[e] = i < m ? sh.list[i] : 0;
+        w[e] = i < m ? wt.weight(key_value(key[e])) : 0;
+        if (i < m) sh.all.key[i] = key[e], sh.all.w[i] = w[e];
+        before[e] = above[e] = 0;
+    }
+    __syncthreads();
+    for (int j = 0; j < m; j++) {   // members and mass before each
+        const u64 kj = sh.all.key[j], wj = sh.all.w[j];
+#pragma unroll
+        for (int e = 0; e < EACH; e++)
+            if (e * SP_THREADS < m && kj > key[e]) above[e]++, before[e] += wj;
+    }
+    u64 mass = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; e++)
+        if (tid + e * SP_THREADS < m && above[e] < k) mass += w[e];
+    const double want = (double)p * (double)block_add(mass, sh.part);
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int i = tid + e * SP_THREADS;
+        if (i >= m) break;
+        const bool keep = above[e] < k && (above[e] == 0 || p > 1.0f || (double)before[e] < want) && w[e] >= least;
+        w[e] = keep ? w[e] : 0;
+        kept += w[e];
+        sh.list[i] = (u64)argmax_key_index(key[e]) << 44 | w[e];   // a weight has at most 44 bits, an index 18
+    }
+    const u64 total = block_add(kept, sh.part), goal = sample_goal(u, total);
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const int i = tid + e * SP_THREADS;
+        if (i >= m || !w[e]) continue;
+        const u64 mine = sh.list[i];
+        u64 run = 0;   // the kept weights at lower indexes
+        for (int j = 0; j < m; j++) {
+            const u64 o = sh.list[j];
+            run += o < mine ? o & ((1ull << 44) - 1) : 0;
+        }
+        if (goal >= run && goal < run + w[e]) a.tokens[row] = (int)(mine >> 44);
+    }
+}
+
 template <typename T, int CL>
 __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int slice) {
     extern __shared__ __align__(16) char sp_smem[];
@@ -276,78 +370,143 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     const int rank = (int)cl.block_rank(), row = blockIdx.x / CL;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int first = min(a.vocab, rank * slice), n = min(slice, a.vocab - first);
+    cl.barrier_arrive();   // this CTA runs: the others may write to its shared memory
 
-    // The slice into shared memory, at the same offset from a 16-byte boundary as in memory.
+    // The slice into shared memory, at the same offset from a 16-byte boundary
+    // as in memory; NaN becomes -inf.
     const T *src = (const T *)a.logits + row * a.stride + first;
     constexpr int N = Vec16<T>::N;
-    const int shift = (int)(((uintptr_t)src & 15) / sizeof(T));
-    T *x = (T *)(sp_smem + sizeof(SampleShared)) + shift;
-    u64 best = 0;
-    {
-        float top = -INFINITY;
-        int at = -1;
+    const int shift = (int)(((uintptr_t)src & 15) / sizeof(T)), vecs = (n + shift + N - 1) / N;
+    Vec16<T> *x = (Vec16<T> *)(sp_smem + sizeof(SampleShared));
+    float most = -INFINITY;   // of this thread
 #pragma unroll 4
-        for (int v = tid; v * N < n + shift; v += SP_THREADS) {
-            const int i0 = v * N - shift;
-            if (i0 >= 0 && i0 + N <= n) {
-                const Vec16<T> e = *(const Vec16<T> *)(src + i0);
-                *(Vec16<T> *)(x + i0) = e;
+    for (int v = tid; v < vecs; v += SP_THREADS) {
+        const int i0 = v * N - shift;
+        Vec16<T> e;
+        if (i0 >= 0 && i0 + N <= n) {
+            e = *(const Vec16<T> *)(src + i0);
+        } else {
 #pragma unroll
-                for (int k = 0; k < N; k++) {
-                    const float f = logit(e.e[k]);
-                    if (f > top || at < 0) top = f, at = i0 + k;
-                }
-            } else {
-                for (int k = max(0, -i0); k < N && i0 + k < n; k++) {
-                    const T e = src[i0 + k];
-                    x[i0 + k] = e;
-                    const float f = logit(e);
-                    if (f > top || at < 0) top = f, at = i0 + k;
-                }
-            }
+            for (int k = 0; k < N; k++) e.e[k] = i0 + k >= 0 && i0 + k < n ? src[i0 + k] : Elem<T>::down(-INFINITY);
         }
-        if (at >= 0) best = argmax_key(top, first + at);
+        bool odd = false;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float f = Elem<T>::up(e.e[k]);
+            odd |= f != f;
+            most = fmaxf(most, f);   // of a NaN and a number, the number
+        }
+        if (odd)
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (Elem<T>::up(e.e[k]) != Elem<T>::up(e.e[k])) e.e[k] = Elem<T>::down(-INFINITY);
+        x[v] = e;
     }
     for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
     if (tid < 32) sh.table[tid] = exp2((double)tid / 32.0);
     const float temp = a.temperature ? a.temperature[row] : 1.0f;
     const int want_k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-    SampleRow<T, CL> R = {sh, cl, x, n, first, rank, {}, 0};
-    best = warp_top(best);
-    if (lane == 0) sh.part[warp] = best;
-    if (tid == 0) sh.lo = sh.hi = sh.border[1] = ~0ull;
-    cl.sync();   // every CTA of the cluster runs: its shared memory may be written
+    SampleRow<T, CL> R = {sh, cl, x, vecs, first - shift, rank, {}, 0};
+    float top = warp_max(most);
+    if (lane == 0) sh.part[warp] = __float_as_uint(top);
+    if (tid == 0) sh.lo = sh.hi = sh.border[1] = ~0ull, sh.n_few = 0;
+    __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SP_WARPS; w++) best = max(best, sh.part[w]);
-    R.push(IN_BEST, best);
+    for (int w = 0; w < SP_WARPS; w++) top = fmaxf(top, __uint_as_float((unsigned)sh.part[w]));
+    cl.barrier_wait();
+    R.push(IN_BEST, __float_as_uint(top));
     cl.sync();
 #pragma unroll
-    for (int q = 0; q < CL; q++) best = max(best, sh.in[IN_BEST][q]);
-
-    const float top = key_value(best);
-    if (top == -INFINITY || !(temp > 0.0f)) {
-        if (tid == 0 && rank == 0) a.tokens[row] = top == -INFINITY ? -1 : argmax_key_index(best);
+    for (int q = 0; q < CL; q++) top = fmaxf(top, __uint_as_float((unsigned)sh.in[IN_BEST][q]));
+    top += 0.0f;
+    if (top == -INFINITY) {
+        if (tid == 0 && rank == 0) a.tokens[row] = -1;
+        return;
+    }
+    if (!(temp > 0.0f) || want_k == 1) {   // the first maximum
+        int at = INT_MAX;
+        if (most == top) R.each([&](float v, int i) { at = v == top ? min(at, i) : at; });
+        at = __reduce_min_sync(0xffffffffu, at);
+        __syncthreads();
+        if (lane == 0) sh.part[warp] = at;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < SP_WARPS; w++) at = min(at, (int)sh.part[w]);
+        R.push(IN_MASS, at);
+        cl.sync();
+#pragma unroll
+        for (int q = 0; q < CL; q++) at = min(at, (int)sh.in[IN_MASS][q]);
+        if (tid == 0 && rank == 0) a.tokens[row] = at;
         return;
     }
     const double c = 1.4426950408889634 / (double)temp;
-    const Weigh wt = {top, (float)((SP_BINS - 1) / SP_RANGE * c), c, (double)top * c, sh.table};
+    const Weigh wt = {top, fmaxf((float)((SP_BINS - 1) / SP_RANGE * c), 1e-30f), c, (double)top * c, sh.table};
     R.wt = wt;
     const bool by_k = want_k > 0 && want_k < a.vocab, by_p = p < 1.0f;
-    u64 floor_key = 0;   // tokens with a key at or above it are kept
+    const double least_w = ceil((mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE);
+    const u64 least = least_w > 0 ? (u64)least_w : 0;   // min_p as a weight
+    const u64 best = order_key(top, 0);   // at or above every key
+    Floor floor = {-INFINITY, INT_MAX};
 
+    if (by_k && want_k <= SP_FEW) {
+        // The bin in which k of the threads' maxima lie: at least k logits are in it or before it.
+        const int mb = Weigh::bin(wt.place(most));
+        if (mb < SP_BINS - 1) atomicAdd(&sh.hist[mb], 1u);
+        cl.sync();
+        constexpr int PER = SP_BINS / CL / SP_THREADS;
+        const int bin0 = (rank * SP_THREADS + tid) * PER;
+        int cnt[PER], mine = 0, own;
+        R.template gather<PER>(sh.hist, bin0, cnt);
+#pragma unroll
+        for (int i = 0; i < PER; i++) mine += cnt[i];
+        int before = block_scan(mine, (int *)sh.part, own);
+        R.push(IN_FEW, own);
+        cl.sync();
+        before += (int)R.pushed_before(IN_FEW);
+        const bool found = (int)R.pushed(IN_FEW) >= want_k;
+        if (found) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (before < want_k && before + cnt[i] >= want_k)
+                    for (int q = 0; q < CL; q++) *cl.map_shared_rank(&sh.border[0], q) = (u64)(bin0 + i);
+                before += cnt[i];
+            }
+            for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
+            cl.sync();
+            const float edge = (float)((int)sh.border[0] + 1);
+            unsigned *count = cl.map_shared_rank(&sh.n_few, 0);
+            u64 *list = cl.map_shared_rank(sh.list, 0);
+            if (!(wt.place(most) >= edge))
+                R.each([&](float v, int i) {
+                    if (!(wt.place(v) >= edge)) {
+                        const unsigned at = atomicAdd(count, 1u);
+                        if (at < SP_LIST) list[at] = order_key(v, i);
+                    }
+                });
+            cl.sync();
+            const unsigned m = *count;
+            if (m <= SP_LIST) {
+                if (rank > 0) return;
+                few_tokens(a, sh, wt, row, (int)m, want_k, by_p ? p : 2.0f, least, u);
+                cl.sync();   // not before the others have read the count and left
+                return;
+            }
+        } else {
+            for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
+            cl.sync();
+        }
+    }
     if (by_k || by_p) {
         // counts of the bins; with top_p alone, the mass of the row
         u64 mass = 0;
-#pragma unroll 4
-        for (int i = tid; i < n; i += SP_THREADS) {
-            const float v = logit(x[i]);
-            const int b = Weigh::bin(wt.place(v));
-            if (b < SP_BINS - 1) {
-                atomicAdd(&sh.hist[b], 1u);
+        R.each([&](float v, int) {
+            const float f = wt.place(v);
+            if (Weigh::heavy(f)) {
+                atomicAdd(&sh.hist[(int)f], 1u);
                 if (!by_k) mass += wt.weight(v);
             }
-        }
+        });
         R.push(IN_MASS, block_add(mass, sh.part));
         cl.sync();
         u64 total = R.pushed(IN_MASS);
@@ -355,14 +514,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
         constexpr int PER = SP_BINS / CL / SP_THREADS;
         const int bin0 = (rank * SP_THREADS + tid) * PER;
         int cnt[PER], mine = 0;
-#pragma unroll
-        for (int i = 0; i < PER; i++) cnt[i] = 0;
-#pragma unroll
-        for (int q = 0; q < CL; q++) {
-            const unsigned *h = cl.map_shared_rank(sh.hist, (rank + q) % CL) + bin0;   // not all from the same CTA at once
-#pragma unroll
-            for (int i = 0; i < PER; i++) cnt[i] += h[i];
-        }
+        R.template gather<PER>(sh.hist, bin0, cnt);
 #pragma unroll
         for (int i = 0; i < PER; i++) mine += cnt[i];
         if (by_k) {
@@ -384,8 +536,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 const int rest = want_k - (int)(sh.border[0] >> 20 & 0xfffff);   // of the bin's members
                 u64 over = 0;
                 if (in_bin <= SP_LIST) {
-                    const int m = R.collect([&](u64, float f) { return Weigh::bin(f) == bk; },
-                                            [&](float v, u64, float f) { return by_p && Weigh::bin(f) < bk ? wt.weight(v) : 0; }, over, IN_OVER, 0);
+                    const int m = R.collect([&](float, int, float f) { return Weigh::bin(f) == bk; },
+                                            [&](float v, int, float f) { return by_p && Weigh::bin(f) < bk ? wt.weight(v) : 0; }, over, IN_OVER, 0);
                     for (int i = tid; i < m; i += SP_THREADS) {
                         const u64 e = sh.all.key[i];
                         int above = 0;
@@ -394,16 +546,17 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                         if (above == rest - 1) sh.found = e;
                     }
                     __syncthreads();
-                    floor_key = sh.found;
+                    floor = Floor::of(sh.found);
                     if (by_p) {
                         u64 w = 0;
                         for (int i = tid; i < m; i += SP_THREADS)
-                            if (sh.all.key[i] >= floor_key) w += wt.weight(key_value(sh.all.key[i]));
+                            if (sh.all.key[i] >= sh.found) w += wt.weight(key_value(sh.all.key[i]));
                         total = over + block_add(w, sh.part);
                     }
                 } else {
-                    floor_key = R.bisect_count(want_k, best);
-                    if (by_p) total = R.sum([&](float v, u64 e) { return e >= floor_key ? wt.weight(v) : 0; });
+                    const u64 cut = R.bisect_count(want_k, best);
+                    floor = Floor::of(cut);
+                    if (by_p) total = R.sum([&](float v, u64 e) { return e >= cut ? wt.weight(v) : 0; });
                 }
                 // the counts that are left for top_p
 #pragma unroll
@@ -417,7 +570,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
         }
         if (by_p) {
             const double want = (double)p * (double)total;
-            u64 kept = best;   // the lowest key that is kept; the largest one always is
+            u64 kept;   // the lowest key that is kept; the largest one always is
             if (want > 0) {
                 // bracket from the counts: bins whose mass can hold the border
                 const float q = SP_RANGE / (SP_BINS - 1), goal = (float)(want / SP_ONE);
@@ -471,19 +624,20 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 u64 over = 0;
                 int g_lo = 0, g_hi = SP_BINS2;   // the second histogram's bins that are collected
                 const float g_scale = (float)SP_BINS2 / (float)(b_hi - b_lo + 1);
-                auto sub = [&](float f) { return min(SP_BINS2 - 1, (int)((f - (float)b_lo) * g_scale)); };
-                auto inside = [&](u64 e, float f) { return e >= floor_key && Weigh::bin(f) >= b_lo && Weigh::bin(f) <= b_hi; };
+                auto sub = [&](float f) { return min(SP_BINS2 - 1, (int)((f - (float)b_lo) * g_scale)); };   // NaN: 0
+                const float f_lo = (float)b_lo, f_hi = (float)(b_hi + 1);
+                // place() of an infinite maximum is NaN, which belongs to bin 0
+                auto above = [&](float f) { return b_lo > 0 && !(f >= f_lo); };
+                auto inside = [&](float f) { return !(f >= f_hi) && !above(f); };
                 if (in_range > SP_FEW) {
                     for (int i = tid; i < 3 * SP_BINS2; i += SP_THREADS) ((unsigned *)sh.mass)[i] = 0;
                     __syncthreads();
                     u64 s = 0;
-#pragma unroll 2
-                    for (int i = tid; i < n; i += SP_THREADS) {
-                        const float v = logit(x[i]), f = wt.place(v);
-                        const u64 e = R.key(v, i);
-                        if (e < floor_key || Weigh::bin(f) > b_hi) continue;
+                    R.each([&](float v, int i) {
+                        const float f = wt.place(v);
+                        if (f >= f_hi || !floor.keeps(v, i)) return;
                         const u64 w = wt.weight(v);
-                        if (Weigh::bin(f) < b_lo) {
+                        if (above(f)) {
                             s += w;
                         } else {   // 15 bits at a time: the sums of 2^15 of them stay below 2^30
                             const int g = sub(f);
@@ -491,7 +645,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                             atomicAdd(&sh.mass[1][g], (unsigned)(w >> 15 & 0x7fff));
                             atomicAdd(&sh.mass[2][g], (unsigned)(w >> 30));
                         }
-                    }
+                    });
                     R.push(IN_MASS2, block_add(s, sh.part));
                     cl.sync();
                     const u64 sure = R.pushed(IN_MASS2);
@@ -527,10 +681,9 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 // rank what is left by mass: e is kept while less than the goal is above it
                 int m = SP_LIST + 1;
                 if (g_lo >= 0)
-                    m = R.collect([&](u64 e, float f) { return inside(e, f) && sub(f) >= g_lo && sub(f) < g_hi; },
-                                  [&](float v, u64 e, float f) {
-                                      const int b = Weigh::bin(f);
-                                      return e >= floor_key && (b < b_lo || (b <= b_hi && sub(f) < g_lo)) ? wt.weight(v) : 0;
+                    m = R.collect([&](float v, int i, float f) { return inside(f) && sub(f) >= g_lo && sub(f) < g_hi && floor.keeps(v, i); },
+                                  [&](float v, int i, float f) {
+                                      return (above(f) || (inside(f) && sub(f) < g_lo)) && floor.keeps(v, i) ? wt.weight(v) : 0;
                                   }, over, IN_OVER2, by_k);
                 bool done = false;
                 if (m <= SP_LIST) {
@@ -539,34 +692,39 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                     __syncthreads();
                     for (int i = tid; i < m; i += SP_THREADS) {
                         const u64 e = sh.all.key[i];
-                        u64 above = over;
+                        u64 more = over;
 #pragma unroll 4
-                        for (int j = 0; j < m; j++) above += sh.all.key[j] > e ? sh.all.w[j] : 0;
-                        if ((double)above < want) atomicMin(&sh.found, e);
+                        for (int j = 0; j < m; j++) more += sh.all.key[j] > e ? sh.all.w[j] : 0;
+                        if ((double)more < want) atomicMin(&sh.found, e);
                     }
                     __syncthreads();
                     done = sh.found != ~0ull;
                     if (done) kept = sh.found;
                 }
-                if (!done) kept = R.bisect_mass(want, floor_key, best);
+                if (!done) kept = R.bisect_mass(want, order_key(floor.v, floor.i), best);
+            } else {
+                kept = R.bisect_count(1, best);
             }
-            floor_key = max(floor_key, kept);
+            floor = Floor::of(kept);
         }
     }
 
-    // The kept weights in index order: a warp has a run of the slice.
-    const double least = (mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE;
-    auto kept_weight = [&](int i) -> u64 {
-        const float v = logit(x[i]);
-        if (R.key(v, i) < floor_key) return 0;
+    // The kept weights in index order: a warp has a run of the slice's vectors.
+    auto kept_weight = [&](float v, int i) -> u64 {
+        if (!floor.keeps(v, i)) return 0;
         const u64 w = wt.weight(v);
-        return (double)w < least ? 0 : w;
+        return w < least ? 0 : w;
     };
-    const int run = (n + SP_THREADS - 1) / SP_THREADS * 32;
+    auto kept_vector = [&](int v) -> u64 {
+        const Vec16<T> e = x[v];
+        u64 t = 0;
+#pragma unroll
+        for (int k = 0; k < N; k++) t += kept_weight(Elem<T>::up(e.e[k]), R.first + v * N + k);
+        return t;
+    };
+    const int run = (vecs + SP_THREADS - 1) / SP_THREADS * 32;
     u64 s = 0;
-    const int end = min(n, (warp + 1) * run);
-#pragma unroll 4
-    for (int i = warp * run + lane; i < end; i += 32) s += kept_weight(i);
+    for (int v = warp * run + lane; v < min(vecs, (warp + 1) * run); v += 32) s += kept_vector(v);
     s = warp_add(s);
     __syncthreads();
     if (lane == 0) sh.part[warp] = s;
@@ -577,32 +735,42 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     R.push(IN_KEPT, own);
     cl.sync();   // the last access to another CTA is before it, so each may leave from here on
     const u64 before = R.pushed_before(IN_KEPT), total = R.pushed(IN_KEPT);
-    const double ut = (double)u * (double)total;
-    u64 goal = ut > 0 ? (ut < (double)total ? (u64)ut : total - 1) : 0;
-    if (goal >= total) goal = total - 1;
+    u64 goal = sample_goal(u, total);
     if (goal < before || goal >= before + own) return;
     goal -= before;
     u64 at = 0;
     int w0 = 0;   // the warp's run that holds it
     for (; w0 < SP_WARPS - 1 && at + sh.part[w0] <= goal; w0++) at += sh.part[w0];
-    const int r0 = w0 * run, r1 = min(n, r0 + run);
+    const int r0 = w0 * run, r1 = min(vecs, r0 + run);
     const int piece = (r1 - r0 + SP_THREADS - 1) / SP_THREADS * 32;   // and of that, a piece per warp
+    const int p0 = r0 + warp * piece, p1 = min(r1, p0 + piece);
     s = 0;
-    for (int i = r0 + warp * piece + lane; i < min(r1, r0 + (warp + 1) * piece); i += 32) s += kept_weight(i);
+    for (int v = p0 + lane; v < p1; v += 32) s += kept_vector(v);
     s = warp_add(s);
     if (lane == 0) sh.part2[warp] = s;
     __syncthreads();
     for (int w = 0; w < warp; w++) at += sh.part2[w];
     if (goal < at || goal >= at + s) return;
-    for (int i0 = r0 + warp * piece; i0 < min(r1, r0 + (warp + 1) * piece); i0 += 32) {
-        const u64 w = i0 + lane < r1 ? kept_weight(i0 + lane) : 0;
+    for (int v0 = p0; v0 < p1; v0 += 32) {
+        const int v = v0 + lane;
+        const u64 w = v < p1 ? kept_vector(v) : 0;
         u64 inc = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += y;
         }
-        if (w && goal >= at + inc - w && goal < at + inc) a.tokens[row] = first + i0 + lane;
+        if (goal >= at + inc - w && goal < at + inc) {   // this lane's vector holds it
+            u64 c0 = at + inc - w;
+            const Vec16<T> e = x[v];
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const int i = R.first + v * N + k;
+                const u64 wk = kept_weight(Elem<T>::up(e.e[k]), i);
+                if (goal >= c0 && goal < c0 + wk) a.tokens[row] = i;
+                c0 += wk;
+            }
+        }
         at += __shfl_sync(0xffffffffu, inc, 31);
     }
 }
@@ -619,7 +787,7 @@ static int sample_cluster(int rows, int vocab, int n_sm) {
 template <typename T, int CL>
 static cudaError_t launch_sample_cl(const ptc_sample_args &a, cudaStream_t s) {
     const int slice = (a.vocab + CL - 1) / CL;
-    const size_t smem = sizeof(SampleShared) + (size_t)slice * sizeof(T) + 32;
+    const size_t smem = sizeof(SampleShared) + ((size_t)slice * sizeof(T) + 47) / 16 * 16;   // with the odd ends
     cudaError_t e = cudaFuncSetAttribute(k_sample<T, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
