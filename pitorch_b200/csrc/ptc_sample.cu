@@ -12,16 +12,14 @@
 // rules.
 //
 // Otherwise:
-//  1. a histogram of the logits by their distance from the maximum (4096 bins
-//     of equal width down to where a weight is zero), added up through
-//     distributed shared memory. The bin that holds the k-th largest is
-//     collected and its members ranked: the threshold of top_k;
-//  2. top_p: a bin's mass lies between its count times its lowest and highest
-//     weight, 0.8% apart, so the counts alone bracket the bins in which the
-//     mass can reach top_p times the total. The mass before the bracket is
-//     summed exactly; inside it, the ranking of its members, after a second
-//     histogram of exact masses (1024 bins) where they are many, finds the
-//     last one kept;
+//  1. top_k: a histogram of the logits by their distance from the maximum
+//     (2048 bins of equal width down to the lowest logit that has weight),
+//     added up through distributed shared memory. The bin that holds the k-th
+//     largest is collected and its members ranked: the threshold;
+//  2. top_p: the same with exact masses in place of counts (three sums of 15
+//     bits each, as shared memory adds 32 bits at a time). The bin in which
+//     the mass reaches top_p times the total is collected, and ranking its
+//     members finds the last one kept;
 //  3. min_p is a comparison with the weight, and the token is found from the
 //     kept sums of the CTAs, of their warps and of one warp's elements.
 // Where a bin has too many members to be ranked (equal logits by the
@@ -30,7 +28,7 @@
 // Weights are integers in units of 2^-43 of the largest, so every sum is
 // exact, the order of the atomics has no effect, and the same row gives the
 // same token in any batch. They are computed in 64-bit arithmetic (2^y by a
-// table of 32 and a polynomial of degree 5, relative error below 2^-45): the
+// table of 256 and a polynomial of degree 3, relative error below 2^-42): the
 // running sum of 10^5 weights has to be exact to far better than the weight
 // of one token, which 32-bit exponentials do not give.
 #include <cooperative_groups.h>
@@ -43,32 +41,26 @@ namespace cg = cooperative_groups;
 
 constexpr int SP_THREADS = 512;
 constexpr int SP_WARPS = SP_THREADS / 32;
-constexpr int SP_BINS = 4096;     // of the first histogram; the last one holds what has no weight
-constexpr int SP_BINS2 = 1024;    // of the second
+constexpr int SP_BINS = 2048;
 constexpr int SP_LIST = 1024;     // members that are ranked
-constexpr int SP_FEW = 512;       // ... without a second histogram
+constexpr int SP_FEW = 512;       // top_k up to here by the threads' maxima
 constexpr int SP_SLICE = 16384;   // logits of a CTA, while 8 of them hold the row
 constexpr float SP_RANGE = 44.f;  // weights below 2^-44 are zero
 typedef unsigned long long u64;
 // values that the CTAs of a row tell each other, a slot each
-enum { IN_BEST, IN_FEW, IN_MASS, IN_COUNT, IN_OVER, IN_LIST, IN_BRACKET, IN_RANGE, IN_BEFORE, IN_MASS2, IN_SEG2, IN_OVER2, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
+enum { IN_BEST, IN_FIRST, IN_FEW, IN_COUNT, IN_LIST, IN_MASS, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
 constexpr double SP_ONE = 8796093022208.0;   // 2^43
 
 struct alignas(16) SampleShared {
-    unsigned hist[SP_BINS];
-    // the second histogram (sums of the weights' low, middle and high 15 bits),
-    // or a list of all CTAs' members with their weights
-    union {
-        unsigned mass[3][SP_BINS2];
-        struct {
-            u64 key[SP_LIST], w[SP_LIST];
-        } all;
-    };
-    u64 list[SP_LIST];   // this CTA's members
-    double table[32];    // 2^(j/32)
+    unsigned hist[3][SP_BINS];   // counts in the first, or the low, middle and high 15 bits of masses
+    struct {
+        u64 key[SP_LIST], w[SP_LIST];
+    } all;               // the members of all CTAs, with their weights
+    u64 list[SP_LIST];   // this CTA's
+    double table[256];   // 2^(j/256)
     u64 in[SP_SLOTS][8];   // what each CTA of the cluster pushed here, by value and rank
     u64 part[SP_WARPS], part2[SP_WARPS];
-    u64 border[2], found, lo, hi;
+    u64 border[2], found;
     unsigned n_list, n_few;
 };
 
@@ -89,30 +81,28 @@ __device__ __forceinline__ double widen(float x) {
 
 // How a row's logits become bins and weights.
 struct Weigh {
-    float top, scale;   // bins per unit of distance
+    float top, most;    // the maximum, and the distance from it at which weights become zero
+    float scale;        // bins per unit of distance
     double c, topc;     // log2(e) / temperature, and times the maximum
     const double *table;
 
-    // Distance from the maximum in bins; NaN for an infinite maximum itself.
-    __device__ float place(float x) const { return (top - x) * scale; }
-    __device__ static bool heavy(float f) { return !(f >= (float)(SP_BINS - 1)); }   // has weight
-    __device__ static int bin(float f) { return heavy(f) ? (int)f : SP_BINS - 1; }
-    // 2^y for y = (x - top) log2(e) / temperature: y = n/32 + r, 2^(n/32) from
-    // the table and the exponent, 2^r by its series (ln 2)^i / i!
+    // (the distance of an infinite maximum from itself is NaN: heavy, in bin 0)
+    __device__ bool heavy(float x) const { return !(top - x >= most); }
+    __device__ int bin(float x) const { return min(SP_BINS - 1, (int)((top - x) * scale)); }
+    // 2^y for y = (x - top) log2(e) / temperature: y = n/256 + r, 2^(n/256)
+    // from the table and the exponent, 2^r by its series (ln 2)^i / i!, to 2^-42
     __device__ u64 weight(float x) const {
-        if (!heavy(place(x))) return 0;
+        if (!heavy(x)) return 0;
         if (x == top) return 1ull << 43;
         const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the rounded integer
-        const double y = fma(widen(x), c, -topc), t = fma(y, 32.0, magic);
+        const double y = fma(widen(x), c, -topc), t = fma(y, 256.0, magic);
         const int n = __double2loint(t);
-        const double r = fma(t - magic, -1.0 / 32.0, y);
-        double p = 1.3333558146428443e-3;
-        p = fma(p, r, 9.618129107628477e-3);
-        p = fma(p, r, 5.550410866482158e-2);
+        const double r = fma(t - magic, -1.0 / 256.0, y);
+        double p = 5.550410866482158e-2;
         p = fma(p, r, 2.402265069591007e-1);
         p = fma(p, r, 6.931471805599453e-1);
-        p = fma(p, r, 1.0) * table[n & 31];
-        p = __hiloint2double(__double2hiint(p) + (((n >> 5) + 43) << 20), __double2loint(p));
+        p = fma(p, r, 1.0) * table[n & 255];
+        p = __hiloint2double(__double2hiint(p) + (((n >> 8) + 43) << 20), __double2loint(p));
         return (u64)__double_as_longlong(p + 4503599627370496.0) & ((1ull << 52) - 1);
     }
 };
@@ -213,17 +203,54 @@ struct SampleRow {
         return t;
     }
 
-    // The counts of PER bins from bin0 on, over the cluster.
-    template <int PER>
-    __device__ void gather(unsigned *hist, int bin0, int (&cnt)[PER]) {
+    // A CTA adds up its share of the bins over the cluster, PER to a thread
+    // (where there are fewer bins than threads, the last threads have none).
+    static constexpr int SHARE = SP_BINS / CL, PER = SHARE > SP_THREADS ? SHARE / SP_THREADS : 1;
+    __device__ int bin0() const { return rank * SHARE + threadIdx.x * PER; }
+    template <int PARTS>
+    __device__ void gather(u64 (&sum)[PER]) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) cnt[i] = 0;
+        for (int i = 0; i < PER; i++) sum[i] = 0;
+        if (threadIdx.x * PER >= SHARE) return;
 #pragma unroll
         for (int q = 0; q < CL; q++) {
-            const unsigned *h = cl.map_shared_rank(hist, (rank + q) % CL) + bin0;   // not all from the same CTA at once
+            const unsigned *h = cl.map_shared_rank(&sh.hist[0][0], (rank + q) % CL) + bin0();   // not all from the same CTA at once
 #pragma unroll
-            for (int i = 0; i < PER; i++) cnt[i] += h[i];
+            for (int i = 0; i < PER; i++)
+#pragma unroll
+                for (int k = 0; k < PARTS; k++) sum[i] += (u64)h[k * SP_BINS + i] << (15 * k);
         }
+    }
+    // The bin in which the running sum of the gathered ones reaches `want`, and
+    // the sum before it, into every CTA's sh.border (false: it stays below);
+    // `total` is the sum of all. Two barriers of the cluster.
+    template <typename V>
+    __device__ bool cross(const u64 (&sum)[PER], double share, V want, u64 &total, int slot) {
+        u64 mine = 0, own;
+#pragma unroll
+        for (int i = 0; i < PER; i++) mine += sum[i];
+        u64 before = block_scan(mine, sh.part, own);
+        push(slot, own);
+        cl.sync();
+        before += pushed_before(slot);
+        total = pushed(slot);
+        const double goal = share > 0 ? share * (double)total : (double)want;
+        if ((double)total < goal) return false;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            if ((double)before < goal && (double)(before + sum[i]) >= goal)
+                for (int q = 0; q < CL; q++) {
+                    u64 *to = cl.map_shared_rank(sh.border, q);
+                    to[0] = (u64)(bin0() + i);
+                    to[1] = before;
+                }
+            before += sum[i];
+        }
+        cl.sync();
+        return true;
+    }
+    __device__ void clear(int parts) {
+        for (int i = threadIdx.x; i < parts * SP_BINS / 4; i += SP_THREADS) ((uint4 *)&sh.hist[0][0])[i] = make_uint4(0, 0, 0, 0);
     }
 
     // Sum over the cluster of f(value, key), a barrier of the cluster in it.
@@ -260,43 +287,33 @@ struct SampleRow {
         return lo;
     }
 
-    // Collects the keys of what `in` picks and sums `add` over the rest of the row;
-    // one barrier of the cluster. Every CTA then has all of them in sh.all.key
-    // (their number is returned; more than SP_LIST: nothing to use). The two
-    // calls of a row use a list each, as the other CTAs may still read the
-    // first when the second begins; the second's takes the place of the first
-    // histogram, which everyone has read by then.
-    template <typename In, typename Add>
-    __device__ int collect(In in, Add add, u64 &total, int slot, int second) {
-        static_assert(sizeof(sh.hist) >= sizeof(sh.list), "the second list fits");
-        u64 *list = second ? (u64 *)sh.hist : sh.list;
+    // Collects the keys of what `in` picks; one barrier of the cluster. Every
+    // CTA then has all of them in sh.all.key (their number is returned; more
+    // than SP_LIST: nothing to use). The two calls of a row have a barrier of
+    // the cluster between them, after which nobody reads the first list.
+    template <typename In>
+    __device__ int collect(In in, int slot) {
         if (threadIdx.x == 0) sh.n_list = 0;
         __syncthreads();
-        u64 s = 0;
         each([&](float v, int i) {
-            const float f = wt.place(v);
-            if (in(v, i, f)) {
+            if (in(v, i)) {
                 const unsigned at = atomicAdd(&sh.n_list, 1u);
-                if (at < SP_LIST) list[at] = order_key(v, i);
-            } else {
-                s += add(v, i, f);
+                if (at < SP_LIST) sh.list[at] = order_key(v, i);
             }
         });
-        s = block_add(s, sh.part);
-        push(slot, s);
-        push(slot + 1, min(sh.n_list, (unsigned)SP_LIST + 1));
+        __syncthreads();
+        push(slot, min(sh.n_list, (unsigned)SP_LIST + 1));
         cl.sync();
-        total = pushed(slot);
-        const int m = (int)pushed(slot + 1);
+        const int m = (int)pushed(slot);
         if (m <= SP_LIST) {
             for (int i = threadIdx.x; i < m; i += SP_THREADS) {
                 int q = 0, at = i;   // member i is the at-th of CTA q
 #pragma unroll
                 for (int k = 0; k < CL - 1; k++) {
-                    const int c = (int)sh.in[slot + 1][k];
+                    const int c = (int)sh.in[slot][k];
                     if (q == k && at >= c) at -= c, q++;
                 }
-                sh.all.key[i] = cl.map_shared_rank(list, q)[at];
+                sh.all.key[i] = cl.map_shared_rank(sh.list, q)[at];
             }
             __syncthreads();
         }
@@ -378,7 +395,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     constexpr int N = Vec16<T>::N;
     const int shift = (int)(((uintptr_t)src & 15) / sizeof(T)), vecs = (n + shift + N - 1) / N;
     Vec16<T> *x = (Vec16<T> *)(sp_smem + sizeof(SampleShared));
-    float most = -INFINITY;   // of this thread
+    float most = -INFINITY, lowest = INFINITY;   // of this thread; -inf left out of the second
 #pragma unroll 4
     for (int v = tid; v < vecs; v += SP_THREADS) {
         const int i0 = v * N - shift;
@@ -395,6 +412,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
             const float f = Elem<T>::up(e.e[k]);
             odd |= f != f;
             most = fmaxf(most, f);   // of a NaN and a number, the number
+            lowest = fminf(lowest, f == -INFINITY ? INFINITY : f);
         }
         if (odd)
 #pragma unroll
@@ -402,23 +420,30 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 if (Elem<T>::up(e.e[k]) != Elem<T>::up(e.e[k])) e.e[k] = Elem<T>::down(-INFINITY);
         x[v] = e;
     }
-    for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
-    if (tid < 32) sh.table[tid] = exp2((double)tid / 32.0);
+    if (tid < 256) sh.table[tid] = exp2((double)tid / 256.0);
     const float temp = a.temperature ? a.temperature[row] : 1.0f;
     const int want_k = a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, mp = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
     SampleRow<T, CL> R = {sh, cl, x, vecs, first - shift, rank, {}, 0};
+    R.clear(3);
     float top = warp_max(most);
-    if (lane == 0) sh.part[warp] = __float_as_uint(top);
-    if (tid == 0) sh.lo = sh.hi = sh.border[1] = ~0ull, sh.n_few = 0;
+    lowest = -warp_max(-lowest);
+    if (lane == 0) sh.part[warp] = (u64)__float_as_uint(lowest) << 32 | __float_as_uint(top);
+    if (tid == 0) sh.n_few = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SP_WARPS; w++) top = fmaxf(top, __uint_as_float((unsigned)sh.part[w]));
+    for (int w = 0; w < SP_WARPS; w++) {
+        top = fmaxf(top, __uint_as_float((unsigned)sh.part[w]));
+        lowest = fminf(lowest, __uint_as_float((unsigned)(sh.part[w] >> 32)));
+    }
     cl.barrier_wait();
-    R.push(IN_BEST, __float_as_uint(top));
+    R.push(IN_BEST, (u64)__float_as_uint(lowest) << 32 | __float_as_uint(top));
     cl.sync();
 #pragma unroll
-    for (int q = 0; q < CL; q++) top = fmaxf(top, __uint_as_float((unsigned)sh.in[IN_BEST][q]));
+    for (int q = 0; q < CL; q++) {
+        top = fmaxf(top, __uint_as_float((unsigned)sh.in[IN_BEST][q]));
+        lowest = fminf(lowest, __uint_as_float((unsigned)(sh.in[IN_BEST][q] >> 32)));
+    }
     top += 0.0f;
     if (top == -INFINITY) {
         if (tid == 0 && rank == 0) a.tokens[row] = -1;
@@ -433,15 +458,17 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < SP_WARPS; w++) at = min(at, (int)sh.part[w]);
-        R.push(IN_MASS, at);
+        R.push(IN_FIRST, at);
         cl.sync();
 #pragma unroll
-        for (int q = 0; q < CL; q++) at = min(at, (int)sh.in[IN_MASS][q]);
+        for (int q = 0; q < CL; q++) at = min(at, (int)sh.in[IN_FIRST][q]);
         if (tid == 0 && rank == 0) a.tokens[row] = at;
         return;
     }
     const double c = 1.4426950408889634 / (double)temp;
-    const Weigh wt = {top, fmaxf((float)((SP_BINS - 1) / SP_RANGE * c), 1e-30f), c, (double)top * c, sh.table};
+    // bins down to the lowest logit or to where weights end, whichever is nearer
+    const float reach = fmaxf((float)(SP_RANGE / c), 1e-37f), spread = fminf(top - lowest, reach);
+    const Weigh wt = {top, reach, spread > 0.f ? fminf((SP_BINS - 1) / spread, 1e30f) : 1e30f, c, (double)top * c, sh.table};
     R.wt = wt;
     const bool by_k = want_k > 0 && want_k < a.vocab, by_p = p < 1.0f;
     const double least_w = ceil((mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE);
@@ -449,37 +476,22 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     const u64 best = order_key(top, 0);   // at or above every key
     Floor floor = {-INFINITY, INT_MAX};
 
+    u64 sums[SampleRow<T, CL>::PER], total;
+
     if (by_k && want_k <= SP_FEW) {
         // The bin in which k of the threads' maxima lie: at least k logits are in it or before it.
-        const int mb = Weigh::bin(wt.place(most));
-        if (mb < SP_BINS - 1) atomicAdd(&sh.hist[mb], 1u);
+        if (wt.heavy(most)) atomicAdd(&sh.hist[0][wt.bin(most)], 1u);
         cl.sync();
-        constexpr int PER = SP_BINS / CL / SP_THREADS;
-        const int bin0 = (rank * SP_THREADS + tid) * PER;
-        int cnt[PER], mine = 0, own;
-        R.template gather<PER>(sh.hist, bin0, cnt);
-#pragma unroll
-        for (int i = 0; i < PER; i++) mine += cnt[i];
-        int before = block_scan(mine, (int *)sh.part, own);
-        R.push(IN_FEW, own);
-        cl.sync();
-        before += (int)R.pushed_before(IN_FEW);
-        const bool found = (int)R.pushed(IN_FEW) >= want_k;
+        R.template gather<1>(sums);
+        const bool found = R.cross(sums, 0.0, want_k, total, IN_FEW);
+        R.clear(1);
         if (found) {
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                if (before < want_k && before + cnt[i] >= want_k)
-                    for (int q = 0; q < CL; q++) *cl.map_shared_rank(&sh.border[0], q) = (u64)(bin0 + i);
-                before += cnt[i];
-            }
-            for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
-            cl.sync();
-            const float edge = (float)((int)sh.border[0] + 1);
+            const int edge = (int)sh.border[0];
             unsigned *count = cl.map_shared_rank(&sh.n_few, 0);
             u64 *list = cl.map_shared_rank(sh.list, 0);
-            if (!(wt.place(most) >= edge))
+            if (wt.bin(most) <= edge)
                 R.each([&](float v, int i) {
-                    if (!(wt.place(v) >= edge)) {
+                    if (wt.bin(v) <= edge) {
                         const unsigned at = atomicAdd(count, 1u);
                         if (at < SP_LIST) list[at] = order_key(v, i);
                     }
@@ -492,221 +504,70 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 cl.sync();   // not before the others have read the count and left
                 return;
             }
-        } else {
-            for (int i = tid; i < SP_BINS / 4; i += SP_THREADS) ((uint4 *)sh.hist)[i] = make_uint4(0, 0, 0, 0);
-            cl.sync();
         }
+        __syncthreads();
     }
-    if (by_k || by_p) {
-        // counts of the bins; with top_p alone, the mass of the row
-        u64 mass = 0;
+    if (by_k) {
         R.each([&](float v, int) {
-            const float f = wt.place(v);
-            if (Weigh::heavy(f)) {
-                atomicAdd(&sh.hist[(int)f], 1u);
-                if (!by_k) mass += wt.weight(v);
-            }
+            if (wt.heavy(v)) atomicAdd(&sh.hist[0][wt.bin(v)], 1u);
         });
-        R.push(IN_MASS, block_add(mass, sh.part));
         cl.sync();
-        u64 total = R.pushed(IN_MASS);
-        // each CTA adds up its share of the bins, PER to a thread
-        constexpr int PER = SP_BINS / CL / SP_THREADS;
-        const int bin0 = (rank * SP_THREADS + tid) * PER;
-        int cnt[PER], mine = 0;
-        R.template gather<PER>(sh.hist, bin0, cnt);
-#pragma unroll
-        for (int i = 0; i < PER; i++) mine += cnt[i];
-        if (by_k) {
-            int own;
-            int before = block_scan(mine, (int *)sh.part, own);
-            R.push(IN_COUNT, own);
-            cl.sync();
-            before += (int)R.pushed_before(IN_COUNT);
-            if ((int)R.pushed(IN_COUNT) >= want_k) {   // else all that has weight is among the k largest
-#pragma unroll
-                for (int i = 0; i < PER; i++) {   // the bin in which the count reaches k, to every CTA
-                    if (before < want_k && before + cnt[i] >= want_k)
-                        for (int q = 0; q < CL; q++)
-                            *cl.map_shared_rank(&sh.border[0], q) = (u64)(bin0 + i) << 40 | (u64)before << 20 | (u64)cnt[i];
-                    before += cnt[i];
-                }
-                cl.sync();
-                const int bk = (int)(sh.border[0] >> 40), in_bin = (int)(sh.border[0] & 0xfffff);
-                const int rest = want_k - (int)(sh.border[0] >> 20 & 0xfffff);   // of the bin's members
-                u64 over = 0;
-                if (in_bin <= SP_LIST) {
-                    const int m = R.collect([&](float, int, float f) { return Weigh::bin(f) == bk; },
-                                            [&](float v, int, float f) { return by_p && Weigh::bin(f) < bk ? wt.weight(v) : 0; }, over, IN_OVER, 0);
-                    for (int i = tid; i < m; i += SP_THREADS) {
-                        const u64 e = sh.all.key[i];
-                        int above = 0;
+        R.template gather<1>(sums);
+        if (R.cross(sums, 0.0, want_k, total, IN_COUNT)) {   // else all that has weight is among the k largest
+            const int bk = (int)sh.border[0], rest = want_k - (int)sh.border[1];   // of the bin's members
+            const int m = R.collect([&](float v, int) { return wt.heavy(v) && wt.bin(v) == bk; }, IN_LIST);
+            if (m <= SP_LIST) {
+                for (int i = tid; i < m; i += SP_THREADS) {
+                    const u64 e = sh.all.key[i];
+                    int above = 0;
 #pragma unroll 4
-                        for (int j = 0; j < m; j++) above += sh.all.key[j] > e;
-                        if (above == rest - 1) sh.found = e;
-                    }
-                    __syncthreads();
-                    floor = Floor::of(sh.found);
-                    if (by_p) {
-                        u64 w = 0;
-                        for (int i = tid; i < m; i += SP_THREADS)
-                            if (sh.all.key[i] >= sh.found) w += wt.weight(key_value(sh.all.key[i]));
-                        total = over + block_add(w, sh.part);
-                    }
-                } else {
-                    const u64 cut = R.bisect_count(want_k, best);
-                    floor = Floor::of(cut);
-                    if (by_p) total = R.sum([&](float v, u64 e) { return e >= cut ? wt.weight(v) : 0; });
+                    for (int j = 0; j < m; j++) above += sh.all.key[j] > e;
+                    if (above == rest - 1) sh.found = e;
                 }
-                // the counts that are left for top_p
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    if (bin0 + i == bk) cnt[i] = rest;
-                    if (bin0 + i > bk) cnt[i] = 0;
-                }
-            } else if (by_p) {
-                total = R.sum([&](float v, u64) { return wt.weight(v); });
-            }
-        }
-        if (by_p) {
-            const double want = (double)p * (double)total;
-            u64 kept;   // the lowest key that is kept; the largest one always is
-            if (want > 0) {
-                // bracket from the counts: bins whose mass can hold the border
-                const float q = SP_RANGE / (SP_BINS - 1), goal = (float)(want / SP_ONE);
-                float low = 0.f, high = 0.f, lows[PER], highs[PER];
-                mine = 0;
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const float b = (float)(bin0 + i);
-                    low += lows[i] = cnt[i] * exp2f(-(b + 1.01f) * q);
-                    high += highs[i] = cnt[i] * exp2f(-(b - 0.01f) * q);
-                    mine += cnt[i];
-                }
-                float own_l, own_h;
-                int own;
-                float bl = block_scan(low, (float *)sh.part, own_l), bh = block_scan(high, (float *)sh.part2, own_h);
-                int before = block_scan(mine, (int *)sh.part, own);
-                R.push(IN_BRACKET, (u64)__float_as_uint(own_l) << 32 | __float_as_uint(own_h));
-                R.push(IN_BEFORE, own);
-                cl.sync();
-#pragma unroll
-                for (int r = 0; r < CL; r++)
-                    if (r < rank) bl += __uint_as_float((unsigned)(sh.in[IN_BRACKET][r] >> 32)), bh += __uint_as_float((unsigned)sh.in[IN_BRACKET][r]);
-                before += (int)R.pushed_before(IN_BEFORE);
-                // first bin that may reach the goal, with the count before it; first that must, with the count through it
-                u64 lo = ~0ull, hi = ~0ull;
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    bl += lows[i];
-                    bh += highs[i];
-                    if (lo == ~0ull && bh * 1.0001f >= goal) lo = (u64)(bin0 + i) << 20 | (u64)before;
-                    before += cnt[i];
-                    if (hi == ~0ull && bl * 0.9999f >= goal) hi = (u64)(bin0 + i) << 20 | (u64)before;
-                }
-                const unsigned los = __ballot_sync(0xffffffffu, lo != ~0ull), his = __ballot_sync(0xffffffffu, hi != ~0ull);
-                if (los && lane == __ffs(los) - 1) atomicMin(&sh.lo, lo);
-                if (his && lane == __ffs(his) - 1) atomicMin(&sh.hi, hi);
                 __syncthreads();
-                R.push(IN_RANGE, (sh.lo & 0xffffffffull) << 32 | (sh.hi & 0xffffffffull));
-                cl.sync();
-                unsigned range_lo = ~0u, range_hi = ~0u;
-#pragma unroll
-                for (int r = 0; r < CL; r++) {
-                    range_lo = min(range_lo, (unsigned)(sh.in[IN_RANGE][r] >> 32));
-                    range_hi = min(range_hi, (unsigned)sh.in[IN_RANGE][r]);
-                }
-                const int all = (int)R.pushed(IN_BEFORE);
-                if (range_hi == ~0u) range_hi = (unsigned)(SP_BINS - 2) << 20 | (unsigned)all;
-                if (range_lo == ~0u) range_lo = (unsigned)(SP_BINS - 2) << 20 | (unsigned)all;
-                const int b_lo = (int)(range_lo >> 20), b_hi = max(b_lo, (int)(range_hi >> 20));
-                const int in_range = (int)(range_hi & 0xfffff) - (int)(range_lo & 0xfffff);
-                u64 over = 0;
-                int g_lo = 0, g_hi = SP_BINS2;   // the second histogram's bins that are collected
-                const float g_scale = (float)SP_BINS2 / (float)(b_hi - b_lo + 1);
-                auto sub = [&](float f) { return min(SP_BINS2 - 1, (int)((f - (float)b_lo) * g_scale)); };   // NaN: 0
-                const float f_lo = (float)b_lo, f_hi = (float)(b_hi + 1);
-                // place() of an infinite maximum is NaN, which belongs to bin 0
-                auto above = [&](float f) { return b_lo > 0 && !(f >= f_lo); };
-                auto inside = [&](float f) { return !(f >= f_hi) && !above(f); };
-                if (in_range > SP_FEW) {
-                    for (int i = tid; i < 3 * SP_BINS2; i += SP_THREADS) ((unsigned *)sh.mass)[i] = 0;
-                    __syncthreads();
-                    u64 s = 0;
-                    R.each([&](float v, int i) {
-                        const float f = wt.place(v);
-                        if (f >= f_hi || !floor.keeps(v, i)) return;
-                        const u64 w = wt.weight(v);
-                        if (above(f)) {
-                            s += w;
-                        } else {   // 15 bits at a time: the sums of 2^15 of them stay below 2^30
-                            const int g = sub(f);
-                            atomicAdd(&sh.mass[0][g], (unsigned)(w & 0x7fff));
-                            atomicAdd(&sh.mass[1][g], (unsigned)(w >> 15 & 0x7fff));
-                            atomicAdd(&sh.mass[2][g], (unsigned)(w >> 30));
-                        }
-                    });
-                    R.push(IN_MASS2, block_add(s, sh.part));
-                    cl.sync();
-                    const u64 sure = R.pushed(IN_MASS2);
-                    constexpr int SEG2 = SP_BINS2 / CL, PER2 = SEG2 > SP_THREADS ? SEG2 / SP_THREADS : 1;
-                    const int g0 = rank * SEG2 + tid * PER2;
-                    u64 m[PER2], sum = 0, own_m;
-#pragma unroll
-                    for (int i = 0; i < PER2; i++) m[i] = 0;
-                    if (tid * PER2 < SEG2) {
-#pragma unroll
-                        for (int r = 0; r < CL; r++) {
-                            const unsigned *h = cl.map_shared_rank((unsigned *)sh.mass, (rank + r) % CL) + g0;
-#pragma unroll
-                            for (int i = 0; i < PER2; i++) m[i] += h[i] + ((u64)h[SP_BINS2 + i] << 15) + ((u64)h[2 * SP_BINS2 + i] << 30);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < PER2; i++) sum += m[i];
-                    u64 at = block_scan(sum, sh.part, own_m);
-                    R.push(IN_SEG2, own_m);
-                    cl.sync();
-                    at += sure + R.pushed_before(IN_SEG2);
-#pragma unroll
-                    for (int i = 0; i < PER2; i++) {   // the bin in which the mass reaches the goal, to every CTA
-                        if ((double)at < want && (double)(at + m[i]) >= want)
-                            for (int r = 0; r < CL; r++) *cl.map_shared_rank(&sh.border[1], r) = (u64)(g0 + i);
-                        at += m[i];
-                    }
-                    cl.sync();
-                    g_lo = sh.border[1] == ~0ull ? -1 : (int)sh.border[1];
-                    g_hi = g_lo + 1;
-                }
-                // rank what is left by mass: e is kept while less than the goal is above it
-                int m = SP_LIST + 1;
-                if (g_lo >= 0)
-                    m = R.collect([&](float v, int i, float f) { return inside(f) && sub(f) >= g_lo && sub(f) < g_hi && floor.keeps(v, i); },
-                                  [&](float v, int i, float f) {
-                                      return (above(f) || (inside(f) && sub(f) < g_lo)) && floor.keeps(v, i) ? wt.weight(v) : 0;
-                                  }, over, IN_OVER2, by_k);
-                bool done = false;
-                if (m <= SP_LIST) {
-                    for (int i = tid; i < m; i += SP_THREADS) sh.all.w[i] = wt.weight(key_value(sh.all.key[i]));
-                    if (tid == 0) sh.found = ~0ull;
-                    __syncthreads();
-                    for (int i = tid; i < m; i += SP_THREADS) {
-                        const u64 e = sh.all.key[i];
-                        u64 more = over;
-#pragma unroll 4
-                        for (int j = 0; j < m; j++) more += sh.all.key[j] > e ? sh.all.w[j] : 0;
-                        if ((double)more < want) atomicMin(&sh.found, e);
-                    }
-                    __syncthreads();
-                    done = sh.found != ~0ull;
-                    if (done) kept = sh.found;
-                }
-                if (!done) kept = R.bisect_mass(want, order_key(floor.v, floor.i), best);
+                floor = Floor::of(sh.found);
             } else {
-                kept = R.bisect_count(1, best);
+                floor = Floor::of(R.bisect_count(want_k, best));
             }
-            floor = Floor::of(kept);
         }
+        R.clear(1);
+        __syncthreads();
+    }
+    if (by_p && p > 0.0f) {
+        R.each([&](float v, int i) {
+            if (!wt.heavy(v) || !floor.keeps(v, i)) return;
+            const u64 w = wt.weight(v);   // 15 bits at a time: the sums of 2^15 of them stay below 2^30
+            const int b = wt.bin(v);
+            atomicAdd(&sh.hist[0][b], (unsigned)(w & 0x7fff));
+            if (w >> 15) atomicAdd(&sh.hist[1][b], (unsigned)(w >> 15 & 0x7fff));
+            if (w >> 30) atomicAdd(&sh.hist[2][b], (unsigned)(w >> 30));
+        });
+        cl.sync();
+        R.template gather<3>(sums);
+        R.cross(sums, (double)p, 0, total, IN_MASS);
+        const int bp = (int)sh.border[0];
+        const u64 over = sh.border[1];
+        const double want = (double)p * (double)total;
+        const int m = R.collect([&](float v, int i) { return wt.heavy(v) && wt.bin(v) == bp && floor.keeps(v, i); }, IN_LIST2);
+        if (m <= SP_LIST) {
+            // ranked by mass: a member is kept while less than the goal is before it
+            for (int i = tid; i < m; i += SP_THREADS) sh.all.w[i] = wt.weight(key_value(sh.all.key[i]));
+            if (tid == 0) sh.found = ~0ull;
+            __syncthreads();
+            for (int i = tid; i < m; i += SP_THREADS) {
+                const u64 e = sh.all.key[i];
+                u64 more = over;
+#pragma unroll 4
+                for (int j = 0; j < m; j++) more += sh.all.key[j] > e ? sh.all.w[j] : 0;
+                if ((double)more < want) atomicMin(&sh.found, e);
+            }
+            __syncthreads();
+            floor = Floor::of(sh.found);
+        } else {
+            floor = Floor::of(R.bisect_mass(want, order_key(floor.v, floor.i), best));
+        }
+    } else if (by_p) {
+        floor = Floor::of(R.bisect_count(1, best));   // the largest alone
     }
 
     // The kept weights in index order: a warp has a run of the slice's vectors.
@@ -734,7 +595,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     for (int w = 0; w < SP_WARPS; w++) own += sh.part[w];
     R.push(IN_KEPT, own);
     cl.sync();   // the last access to another CTA is before it, so each may leave from here on
-    const u64 before = R.pushed_before(IN_KEPT), total = R.pushed(IN_KEPT);
+    const u64 before = R.pushed_before(IN_KEPT);
+    total = R.pushed(IN_KEPT);
     u64 goal = sample_goal(u, total);
     if (goal < before || goal >= before + own) return;
     goal -= before;
