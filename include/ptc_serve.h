@@ -39,7 +39,8 @@ enum {
     PTC_SERVE_ERR_TABLE = 2,    /* a sequence needs more than max_pages pages */
     PTC_SERVE_ERR_TOKENS = 4,   /* more new tokens than max_tokens */
     PTC_SERVE_ERR_LENGTH = 8,   /* a negative or inconsistent length */
-    PTC_SERVE_ERR_INDEX = 16    /* a page, slot or position out of range */
+    PTC_SERVE_ERR_INDEX = 16,   /* a page, slot or position out of range */
+    PTC_SERVE_ERR_WAIT = 32     /* a kernel's bounded wait ran out: its results are not valid */
 };
 
 #define PTC_SERVE_MAX_SEQS 4096   /* sequences of one call */

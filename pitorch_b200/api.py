@@ -54,7 +54,7 @@ class pt_backward_buf_t(C.Structure):
 # Serving operators (include/ptc_serve.h). Pointers are device addresses.
 PTC_F32, PTC_F16, PTC_BF16 = 0, 1, 2
 PTC_SERVE_ERR_PAGES, PTC_SERVE_ERR_TABLE, PTC_SERVE_ERR_TOKENS = 1, 2, 4
-PTC_SERVE_ERR_LENGTH, PTC_SERVE_ERR_INDEX = 8, 16
+PTC_SERVE_ERR_LENGTH, PTC_SERVE_ERR_INDEX, PTC_SERVE_ERR_WAIT = 8, 16, 32
 PTC_ATTN_WORKSPACE_BYTES = 64 << 20
 
 

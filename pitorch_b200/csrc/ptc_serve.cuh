@@ -64,16 +64,19 @@ template <typename T>
 struct Elem;
 template <>
 struct Elem<float> {
+    static constexpr int TYPE = PTC_F32;
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
 };
 template <>
 struct Elem<__half> {
+    static constexpr int TYPE = PTC_F16;
     static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
     static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
 };
 template <>
 struct Elem<__nv_bfloat16> {
+    static constexpr int TYPE = PTC_BF16;
     static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };

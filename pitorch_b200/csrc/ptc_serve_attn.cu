@@ -63,15 +63,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
-    const __half2 v = __floats2half2_rn(x, y);
-    return *(const uint32_t *)&v;
-}
-__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-    return *(const uint32_t *)&v;
-}
-
 // A warp's rows of an item on tensor cores: lane l has rows l / 4 and l / 4 + 8.
 template <typename T, int HDP, int MT>
 struct NarrowRows {
@@ -506,12 +497,14 @@ extern "C" int ptc_paged_attention(const ptc_attn_args *p, void *stream) {
     int n_sm = 0;
     SERVE_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, on.device()));
     const int group = a.n_heads / a.cache.n_kv_heads;
-    const long long most = (long long)(a.max_q < 1 ? 1 : a.max_q) * group;
+    const long long most = (long long)(a.max_q < 1 ? 1 : a.max_q) * group;   // rows of a K/V head
     if (a.cache.dtype == PTC_F32) {
         // rows in registers: as many as the longest sequence fills, up to 8
         if (most <= 1) SERVE_CUDA((ptc::launch_narrow_hd<float, 1>(a, group, n_sm, s)));
         else if (most <= 4) SERVE_CUDA((ptc::launch_narrow_hd<float, 4>(a, group, n_sm, s)));
         else SERVE_CUDA((ptc::launch_narrow_hd<float, 8>(a, group, n_sm, s)));
+    } else if (most > 64 && a.scale > 0.f) {
+        SERVE_CUDA(ptc::launch_attn_wide(a, group, n_sm, s));
     } else if (a.cache.dtype == PTC_F16) {
         SERVE_CUDA((ptc::launch_narrow_hd<__half, 16>(a, group, n_sm, s)));
     } else {

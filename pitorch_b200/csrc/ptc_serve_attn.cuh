@@ -180,4 +180,23 @@ __device__ __forceinline__ long long attn_cell(const ptc_attn_args &a, int page,
     return (unsigned)page < (unsigned)a.cache.n_pages ? page * a.cache.page_stride + off * a.cache.token_stride : -1;
 }
 
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *(const uint32_t *)&v;
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t *)&v;
+}
+
+// 2^x by the special function unit (relative error 2^-22; 2^-inf is 0).
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The kernel for many rows (ptc_serve_attn_wide.cu): 16-bit types, scale > 0.
+cudaError_t launch_attn_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s);
+
 }  // namespace ptc

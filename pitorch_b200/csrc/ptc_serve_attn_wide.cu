@@ -1,0 +1,545 @@
+// ptc_serve_attn_wide.cu -- attention of new tokens over a paged KV cache
+// (include/ptc_serve.h): the kernel for many rows per K/V head, 16-bit types.
+//
+// One CTA per SM on tcgen05 tensor cores. An item has 256 rows, as two tiles
+// of 128 that share every K/V tile of 128 keys and take turns: while one
+// tile's scores become probabilities, the tensor cores work for the other.
+//
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per row: scores from
+//                   tensor memory, running maximum and sum, probabilities back
+//                   to tensor memory as the A operand of the second product
+//   warp 8          one thread issues the products: S = Q K^T (128 x 128 per
+//                   tile) and O += P V, in an order in which each S follows
+//                   the product that read the P in the same place
+//   warps 9-10      Q and K tiles into shared memory, warp 11 V tiles: 16-byte
+//                   asynchronous copies, each of its own (page, token), so any
+//                   page size and stride will do, in the 128-byte swizzle that
+//                   the tensor cores read
+// Twelve warps are three to a scheduler, which leaves a thread 168 registers;
+// a thirteenth would leave 128.
+//
+// Tensor memory: S0 | S1 | O0 | O1; P takes the place of the first half of its
+// S. The running maximum is replaced, and O rescaled, only when it rises by
+// more than 2^8 (probabilities and sums are relative to the same value, so
+// nothing is lost: they stay below 2^8 and 2^8 times the keys).
+#include <limits.h>
+
+#include "ptc_serve_attn.cuh"
+
+namespace ptc {
+
+constexpr int WA_ROWS = 256, WA_TILE = 128, WA_KEYS = 128;
+constexpr int WA_THREADS = 12 * 32;
+constexpr int WA_K_WARPS = 2, WA_V_WARPS = 1;   // that load
+constexpr float WA_RISE = 8.f;
+
+// ---- tcgen05 ------------------------------------------------------------------
+
+__device__ __forceinline__ void tm_alloc(unsigned *where, int cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(where)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tm_free(unsigned at, int cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b),
+        "r"(idesc), "r"((int)add)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, uint64_t b, unsigned idesc, bool add) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b),
+        "r"(idesc), "r"((int)add)
+        : "memory");
+}
+// 32 columns of this warp's 32 lanes. The values may be used after tm_wait_ld on them.
+__device__ __forceinline__ void tm_ld32(uint32_t (&r)[32], unsigned at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+// (the registers pass through it, so that no use moves before it)
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tm_st32(unsigned at, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand in the 128-byte swizzle: 16-bit elements in blocks of
+// 64 columns (128 bytes a row), 8 rows an atom of 1024 bytes.
+//   along K (rows are M or N): atoms `1024` apart
+//   along M/N (rows are K, V as it lies in memory): blocks of 64 `lbo` apart,
+//   groups of 8 rows 1024 apart
+__device__ __forceinline__ uint64_t operand(unsigned at, unsigned lbo) {
+    return (uint64_t)((at >> 4) & 0x3fff) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor: f32 accumulator, 16-bit A and B, 128 rows; b_mn: B's columns are contiguous.
+template <typename T>
+__device__ __forceinline__ unsigned instruction(int n, bool b_mn) {
+    const unsigned f = Elem<T>::TYPE == PTC_BF16 ? 1 : 0;
+    return 1u << 4 | f << 7 | f << 10 | (unsigned)b_mn << 16 | (unsigned)(n >> 3) << 17 | (unsigned)(WA_TILE >> 4) << 24;
+}
+
+// ---- the kernel -----------------------------------------------------------------
+
+struct WideBars {
+    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], done;
+};
+
+struct WideShared {
+    WideBars bar;
+    unsigned bad[4][4];   // keys of a K tile whose page is out of range
+    unsigned tmem;
+    int gave_up;
+    int last;
+    long long scratch[WA_THREADS / 32];
+};
+
+template <int HDP>
+struct WideShape {
+    static constexpr int Q = WA_ROWS * HDP * 2, KV = WA_KEYS * HDP * 2;
+    static constexpr int BYTES = Q + 4 * KV;                // Q, two K, two V
+    static constexpr int COLS = 512;                        // of tensor memory
+    static constexpr int SLOT = WA_ROWS * (HDP + 2);        // floats of a workspace slot
+};
+
+// A wait that gives up (and makes every later one give up at once): the
+// kernel then runs to its end, frees its tensor memory, and reports it.
+struct Waiter {
+    volatile int *gave_up;
+    int *err;
+    __device__ void operator()(uint64_t *bar, unsigned parity) const {
+        for (int it = 0; it < 1 << 22; it++) {
+            if (mbar_try_wait(bar, parity)) return;
+            if ((it & 63) == 63 && *gave_up) return;
+        }
+        *gave_up = 1;
+        serve_err(err, PTC_SERVE_ERR_WAIT);
+    }
+};
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// One group's loads: the previous one is handed over (its barrier arrived at,
+// after a fence towards the tensor cores' reads) when the next is under way.
+struct Handover {
+    uint64_t *pending = nullptr;
+    template <int LEFT>
+    __device__ void done() {
+        if (!pending) return;
+        asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(pending);
+        pending = nullptr;
+    }
+    __device__ void issued(uint64_t *bar) {
+        cp_async_commit();
+        done<1>();
+        pending = bar;
+    }
+};
+
+__device__ __forceinline__ void cp16_or_zero(unsigned dst, const void *src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+// Where 16-byte chunk `ch` of row `row` lies in a tile of `rows` rows.
+__device__ __forceinline__ unsigned swizzled(int rows, int row, int ch) {
+    return (unsigned)((ch >> 3) * rows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+}
+
+// The loading warps of one kind (K with Q, or V): WARPS of them, of which this
+// is the w-th. A lane looks up the cells of every 32nd key of its warp's share.
+template <typename T, int HDP, int WARPS, bool KEYS>
+__device__ void load_tiles(const ptc_attn_args &a, int group, const int *pre, int u0, int u1, WideShared &sh, unsigned q_at, unsigned at, int w,
+                           const Waiter &wait) {
+    using S = WideShape<HDP>;
+    constexpr int CH = HDP / 8, SHARE = WA_KEYS / WARPS, LOOKS = SHARE / 32;
+    const int lane = threadIdx.x & 31, hd = a.cache.head_dim;
+    const T *from = (const T *)(KEYS ? a.cache.k : a.cache.v);
+    uint64_t *full = KEYS ? sh.bar.k_full : sh.bar.v_full, *empty = KEYS ? sh.bar.k_empty : sh.bar.v_empty;
+    Handover over;
+    int n = 0, items = 0;   // tiles and items so far
+    for (int u = u0; u < u1; items++) {
+        const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
+        const int seg0 = u - it.first, tiles = min(it.units - seg0, u1 - u);
+        const int *table = a.page_table + (long long)it.r * a.max_pages;
+        const long long head = it.head * a.cache.head_stride;
+        if (KEYS) {
+            over.done<0>();   // the last S of the item before needs its K tile
+            if (items > 0) wait(&sh.bar.q_empty, (items - 1) & 1);
+            for (int x = w * 32 + lane; x < WA_ROWS * CH; x += WARPS * 32) {
+                const int row = x / CH, ch = x % CH, i = it.i0 + row, tok = i / group;
+                const bool real = i < it.i1 && ch * 8 < hd;
+                const long long off = real ? (it.s.q0 + tok) * a.q_stride + (long long)(it.head * group + i - tok * group) * hd + ch * 8 : 0;
+                cp16_or_zero(q_at + (row >> 7) * (S::Q / 2) + swizzled(WA_TILE, row & 127, ch), (const T *)a.q + off, real);
+            }
+            over.issued(&sh.bar.q_full);
+        }
+        for (int j = 0; j < tiles; j++, n++) {
+            const int t0 = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS + w * SHARE + lane;
+            long long cell[LOOKS];
+#pragma unroll
+            for (int g = 0; g < LOOKS; g++) {
+                const int t = t0 + g * 32;
+                const bool want = t < it.hi && t >= it.lo;
+                cell[g] = -1;
+                if (want) {
+                    const int page = t / a.cache.page_size;
+                    cell[g] = attn_cell(a, table[page], t - page * a.cache.page_size);
+                    if (cell[g] < 0) serve_err(a.err, PTC_SERVE_ERR_INDEX);
+                }
+                const unsigned bad = __ballot_sync(0xffffffffu, want && cell[g] < 0);
+                if (KEYS && lane == 0) sh.bad[n & 3][w * LOOKS + g] = bad;
+            }
+            const int s = n & 1;
+            if (n >= 2) wait(&empty[s], ((n >> 1) - 1) & 1);
+            __syncwarp();
+#pragma unroll
+            for (int g = 0; g < LOOKS; g++)
+#pragma unroll
+                for (int i = 0; i < CH; i++) {
+                    const int x = i * 32 + lane, k = x / CH, ch = x % CH;
+                    const long long c = __shfl_sync(0xffffffffu, cell[g], k);
+                    const bool real = c >= 0 && ch * 8 < hd;
+                    cp16_or_zero(at + s * S::KV + swizzled(WA_KEYS, w * SHARE + g * 32 + k, ch), from + (real ? c + head + ch * 8 : 0), real);
+                }
+            over.issued(&full[s]);
+        }
+        u += tiles;
+    }
+    over.done<0>();
+}
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, int group) {
+    using S = WideShape<HDP>;
+    extern __shared__ char wa_raw[];
+    __shared__ WideShared sh;
+    char *wa_smem = wa_raw + (-smem_u32(wa_raw) & 1023);   // the swizzle is by address: whole atoms
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, heads = a.cache.n_kv_heads, hd = a.cache.head_dim;
+    const unsigned q_at = smem_u32(wa_smem), k_at = q_at + S::Q, v_at = k_at + 2 * S::KV;
+    int *pre = (int *)(wa_smem + S::BYTES);
+    unsigned *flags = (unsigned *)a.workspace;
+    float *slots = (float *)((char *)a.workspace + ATTN_FLAG_BYTES);
+
+    attn_prefix<WA_ROWS, WA_KEYS, WA_THREADS>(a, group, pre, sh.scratch);
+    const int total = pre[a.n_seqs] * heads, C = min((int)gridDim.x, total), c = blockIdx.x;
+    if (c >= C) return;
+    const int u0 = attn_first(c, C, total), u1 = attn_first(c + 1, C, total);
+
+    if (tid == 0) {
+        WideBars &b = sh.bar;
+        mbar_init(&b.q_full, WA_K_WARPS * 32);
+        mbar_init(&b.q_empty, 1);
+        mbar_init(&b.done, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&b.k_full[i], WA_K_WARPS * 32);
+            mbar_init(&b.v_full[i], WA_V_WARPS * 32);
+            mbar_init(&b.k_empty[i], 1);
+            mbar_init(&b.v_empty[i], 1);
+            mbar_init(&b.s_full[i], 1);
+            mbar_init(&b.p_full[i], WA_TILE);
+            mbar_init(&b.o_full[i], 1);
+        }
+        sh.gave_up = 0;
+        mbar_init_fence();
+    }
+    if (warp == 8) tm_alloc(&sh.tmem, S::COLS);
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    const unsigned tm = sh.tmem;
+    const Waiter wait = {&sh.gave_up, a.err};
+
+    if (warp >= 9 + WA_K_WARPS) {
+        load_tiles<T, HDP, WA_V_WARPS, false>(a, group, pre, u0, u1, sh, q_at, v_at, warp - 9 - WA_K_WARPS, wait);
+    } else if (warp >= 9) {
+        load_tiles<T, HDP, WA_K_WARPS, true>(a, group, pre, u0, u1, sh, q_at, k_at, warp - 9, wait);
+    } else if (warp == 8) {
+        // ---- products ----
+        if (lane == 0) {
+            const unsigned id_s = instruction<T>(WA_KEYS, false), id_o = instruction<T>(HDP, true);
+            int n = 0, items = 0, pc[2] = {0, 0};
+            auto scores = [&](int t, int s) {   // S_t = Q_t K^T
+#pragma unroll
+                for (int k = 0; k < HDP / 16; k++) {
+                    const unsigned off = (k >> 2) * WA_TILE * 128 + (k & 3) * 32;
+                    tc_mma_ss(tm + t * WA_KEYS, operand(q_at + t * (S::Q / 2) + off, 16), operand(k_at + s * S::KV + off, 16), id_s, k > 0);
+                }
+                tc_commit(&sh.bar.s_full[t]);
+            };
+            for (int u = u0; u < u1; items++) {
+                const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
+                const int tiles = min(it.units - (u - it.first), u1 - u), both = it.i1 - it.i0 > WA_TILE ? 2 : 1;
+                wait(&sh.bar.q_full, items & 1);
+                wait(&sh.bar.k_full[n & 1], (n >> 1) & 1);
+                tc_after_sync();
+                for (int t = 0; t < both; t++) scores(t, n & 1);
+                tc_commit(&sh.bar.k_empty[n & 1]);
+                if (tiles == 1) tc_commit(&sh.bar.q_empty);
+                for (int j = 0; j < tiles; j++, n++) {
+                    const int s = n & 1;
+                    wait(&sh.bar.v_full[s], (n >> 1) & 1);
+                    if (j + 1 < tiles) wait(&sh.bar.k_full[s ^ 1], ((n + 1) >> 1) & 1);
+                    for (int t = 0; t < both; t++) {
+                        wait(&sh.bar.p_full[t], pc[t]++ & 1);
+                        tc_after_sync();
+#pragma unroll
+                        for (int k = 0; k < WA_KEYS / 16; k++)   // O_t += P_t V, 16 keys a step
+                            tc_mma_ts(tm + 2 * WA_KEYS + t * HDP, tm + t * WA_KEYS + k * 8, operand(v_at + s * S::KV + k * 2048, WA_KEYS * 128), id_o,
+                                      j > 0 || k > 0);
+                        if (j + 1 < tiles) scores(t, s ^ 1);
+                        else tc_commit(&sh.bar.o_full[t]);
+                    }
+                    tc_commit(&sh.bar.v_empty[s]);
+                    if (j + 1 < tiles) tc_commit(&sh.bar.k_empty[s ^ 1]);
+                    if (j + 2 == tiles) tc_commit(&sh.bar.q_empty);
+                }
+                u += tiles;
+            }
+            // (every product has been waited for, unless a wait has given up)
+            tc_commit(&sh.bar.done);
+            wait(&sh.bar.done, 0);
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax ----
+        const int t = warp >> 2, row = tid & 127;
+        const unsigned lanes = (unsigned)(warp & 3) << 21;   // this warp's 32 lanes of tensor memory
+        const unsigned s_tm = tm + t * WA_KEYS + lanes, o_tm = tm + 2 * WA_KEYS + t * HDP + lanes;
+        const float scale = a.scale * LOG2E;
+        int n = 0, sc = 0, oc = 0;
+        for (int u = u0; u < u1;) {
+            const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
+            const int seg0 = u - it.first, tiles = min(it.units - seg0, u1 - u), rows = it.i1 - it.i0;
+            const bool active = t * WA_TILE < rows;   // of the tile, the same for its four warps
+            const int i = it.i0 + t * WA_TILE + row, tok = i / group;
+            const bool real = i < it.i1;
+            // rows that are not there see everything: their zeros need no masking
+            const int pos = it.s.pos0 + tok, hi = real ? min(pos + 1, it.s.cap) : INT_MAX, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
+            float m = -INFINITY, l = 0.f;   // the reference of the probabilities, and their sum
+            if (active) {
+                for (int j = 0; j < tiles; j++, sc++) {
+                    const int key0 = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS;
+                    wait(&sh.bar.s_full[t], sc & 1);
+                    __syncwarp();   // (the accesses to tensor memory are the warp's)
+                    tc_after_sync();
+                    const unsigned *bad = sh.bad[(n + j) & 3];
+                    const bool any_bad = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+                    const bool mask = any_bad || __any_sync(0xffffffffu, key0 + WA_KEYS > hi || key0 < lo);
+                    auto hide = [&](uint32_t(&r)[32], int q) {   // what this row does not see of columns 32 q on
+#pragma unroll
+                        for (int k = 0; k < 32; k++) {
+                            const int key = key0 + q * 32 + k;
+                            if (key >= hi || key < lo || (any_bad && (bad[q] >> k & 1))) r[k] = __float_as_uint(-INFINITY);
+                        }
+                    };
+                    uint32_t x[32], y[32];
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        tm_ld32(x, s_tm + q * 32);
+                        tm_ld32(y, s_tm + q * 32 + 32);
+                        tm_wait_ld(x);
+                        tm_wait_ld(y);
+                        if (mask) {
+                            hide(x, q);
+                            hide(y, q + 1);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 32; k++) top = fmaxf(top, fmaxf(__uint_as_float(x[k]), __uint_as_float(y[k])));
+                    }
+                    top *= scale;
+                    const bool rise = top > m + WA_RISE || (m == -INFINITY && top > -INFINITY);
+                    if (j == 0) {
+                        m = top;
+                    } else if (__any_sync(0xffffffffu, rise)) {
+                        // (the S that was waited for follows the last product into O)
+                        const float f = rise ? exp2f(m - top) : 1.f;
+                        if (rise) m = top;
+                        l *= f;
+#pragma unroll
+                        for (int d = 0; d < HDP; d += 32) {
+                            tm_ld32(x, o_tm + d);
+                            tm_wait_ld(x);
+#pragma unroll
+                            for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
+                            tm_st32(o_tm + d, x);
+                        }
+                        tm_wait_st();
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        tm_ld32(x, s_tm + q * 32);
+                        tm_ld32(y, s_tm + q * 32 + 32);
+                        tm_wait_ld(x);
+                        tm_wait_ld(y);
+                        if (mask) {
+                            hide(x, q);
+                            hide(y, q + 1);
+                        }
+                        // rounded to the type for the product with V (their sum is not)
+                        uint32_t p[32];
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) {
+                            const float e0 = exp2_fast(fmaf(__uint_as_float(x[k]), scale, -ref)), e1 = exp2_fast(fmaf(__uint_as_float(x[k + 1]), scale, -ref));
+                            const float e2 = exp2_fast(fmaf(__uint_as_float(y[k]), scale, -ref)), e3 = exp2_fast(fmaf(__uint_as_float(y[k + 1]), scale, -ref));
+                            sum[0] += e0;
+                            sum[1] += e1;
+                            sum[2] += e2;
+                            sum[3] += e3;
+                            p[k / 2] = pack2(e0, e1, T());
+                            p[16 + k / 2] = pack2(e2, e3, T());
+                        }
+                        tm_st32(s_tm + q * 16, p);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tm_wait_st();
+                    tc_before_sync();
+                    mbar_arrive(&sh.bar.p_full[t]);
+                }
+                wait(&sh.bar.o_full[t], oc++ & 1);
+                __syncwarp();
+                tc_after_sync();
+            }
+            n += tiles;
+            const bool whole = tiles == it.units;
+            float *slot = slots + (long long)(2 * c + (seg0 == 0)) * S::SLOT;
+            if (active) {
+                const float inv = l > 0.f ? 1.f / l : 0.f;
+                T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + i - tok * group) * hd;
+                float *part = slot + (t * WA_TILE + row) * HDP;
+#pragma unroll
+                for (int d = 0; d < HDP; d += 32) {
+                    uint32_t x[32];
+                    tm_ld32(x, o_tm + d);
+                    tm_wait_ld(x);
+                    if (real) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            if (d + k < hd && whole) {
+                                uint4 v;
+                                v.x = pack2(__uint_as_float(x[k]) * inv, __uint_as_float(x[k + 1]) * inv, T());
+                                v.y = pack2(__uint_as_float(x[k + 2]) * inv, __uint_as_float(x[k + 3]) * inv, T());
+                                v.z = pack2(__uint_as_float(x[k + 4]) * inv, __uint_as_float(x[k + 5]) * inv, T());
+                                v.w = pack2(__uint_as_float(x[k + 6]) * inv, __uint_as_float(x[k + 7]) * inv, T());
+                                *(uint4 *)(dst + d + k) = v;
+                            } else if (d + k < hd) {
+                                *(uint4 *)(part + d + k) = make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                                *(uint4 *)(part + d + k + 4) = make_uint4(x[k + 4], x[k + 5], x[k + 6], x[k + 7]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!whole && real) {
+                    slot[WA_ROWS * HDP + t * WA_TILE + row] = m;
+                    slot[WA_ROWS * (HDP + 1) + t * WA_TILE + row] = l;
+                }
+                tc_before_sync();
+            }
+            if (!whole) {
+                const int c0 = attn_owner(it.first, C, total), c1 = attn_owner(it.first + it.units - 1, C, total);
+                bar_sync(1, WA_ROWS);
+                if (tid == 0) {
+                    __threadfence();
+                    sh.last = atom_add_acq_rel(&flags[c0], 1u) == (unsigned)(c1 - c0);
+                    __threadfence();
+                }
+                bar_sync(1, WA_ROWS);
+                if (sh.last) {
+                    for (int x = tid; x < rows * (HDP / 8); x += WA_ROWS) {
+                        const int r = x / (HDP / 8), d = x % (HDP / 8) * 8;
+                        if (d >= hd) continue;
+                        float top = -INFINITY, sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                        for (int p = c0; p <= c1; p++) top = fmaxf(top, __ldcg(slots + (long long)(2 * p + (p == c0)) * S::SLOT + WA_ROWS * HDP + r));
+                        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 2
+                        for (int p = c0; p <= c1; p++) {
+                            const float *from = slots + (long long)(2 * p + (p == c0)) * S::SLOT;
+                            const float f = exp2f(__ldcg(from + WA_ROWS * HDP + r) - ref);
+                            sum += f * __ldcg(from + WA_ROWS * (HDP + 1) + r);
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const float4 v = __ldcg((const float4 *)(from + r * HDP + d) + h);
+                                acc[4 * h] += f * v.x;
+                                acc[4 * h + 1] += f * v.y;
+                                acc[4 * h + 2] += f * v.z;
+                                acc[4 * h + 3] += f * v.w;
+                            }
+                        }
+                        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                        const int k = it.i0 + r, tk = k / group;
+                        uint4 v;
+                        v.x = pack2(acc[0] * inv, acc[1] * inv, T());
+                        v.y = pack2(acc[2] * inv, acc[3] * inv, T());
+                        v.z = pack2(acc[4] * inv, acc[5] * inv, T());
+                        v.w = pack2(acc[6] * inv, acc[7] * inv, T());
+                        *(uint4 *)((T *)a.out + (it.s.q0 + tk) * a.out_stride + (long long)(it.head * group + k - tk * group) * hd + d) = v;
+                    }
+                    if (tid == 0) flags[c0] = 0;
+                }
+                bar_sync(1, WA_ROWS);   // before `last` is written again
+            }
+            u += tiles;
+        }
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    if (warp == 8) tm_free(tm, S::COLS);
+}
+
+template <typename T, int HDP>
+static cudaError_t launch_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+    using S = WideShape<HDP>;
+    static_assert(2 * 148 * (long long)S::SLOT * 4 + ATTN_FLAG_BYTES <= (long long)PTC_ATTN_WORKSPACE_BYTES, "two slots for each SM");
+    auto kernel = k_attn_wide<T, HDP>;
+    const int smem = 1024 + S::BYTES + (a.n_seqs + 1) * (int)sizeof(int);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const long long fit = (long long)(PTC_ATTN_WORKSPACE_BYTES - ATTN_FLAG_BYTES) / (2 * S::SLOT * (int)sizeof(float));
+    kernel<<<(unsigned)(n_sm < fit ? n_sm : fit), WA_THREADS, smem, s>>>(a, group);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attn_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+    const bool small = a.cache.head_dim <= 64;
+    if (a.cache.dtype == PTC_F16) return small ? launch_wide<__half, 64>(a, group, n_sm, s) : launch_wide<__half, 128>(a, group, n_sm, s);
+    return small ? launch_wide<__nv_bfloat16, 64>(a, group, n_sm, s) : launch_wide<__nv_bfloat16, 128>(a, group, n_sm, s);
+}
+
+}  // namespace ptc
