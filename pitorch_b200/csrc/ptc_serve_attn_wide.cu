@@ -11,10 +11,12 @@
 //   warp 8          one thread issues the products: S = Q K^T (128 x 128 per
 //                   tile) and O += P V, in an order in which each S follows
 //                   the product that read the P in the same place
-//   warps 9-10      Q and K tiles into shared memory, warp 11 V tiles: 16-byte
-//                   asynchronous copies, each of its own (page, token), so any
-//                   page size and stride will do, in the 128-byte swizzle that
-//                   the tensor cores read
+//   warps 9-10      Q and K tiles into shared memory, warp 11 V tiles, in the
+//                   128-byte swizzle that the tensor cores read: whole tiles by
+//                   TMA, a box per run of tokens that lie in one page (8 to 64),
+//                   what ends inside a tile by 16-byte asynchronous copies with
+//                   zeros behind it, and so do page sizes that are no multiple
+//                   of 8
 // Twelve warps are three to a scheduler, which leaves a thread 168 registers;
 // a thirteenth would leave 128.
 //
@@ -22,7 +24,9 @@
 // S. The running maximum is replaced, and O rescaled, only when it rises by
 // more than 2^8 (probabilities and sums are relative to the same value, so
 // nothing is lost: they stay below 2^8 and 2^8 times the keys).
+#include <cuda.h>
 #include <limits.h>
+#include <string.h>
 
 #include "ptc_serve_attn.cuh"
 
@@ -178,10 +182,24 @@ __device__ __forceinline__ unsigned swizzled(int rows, int row, int ch) {
     return (unsigned)((ch >> 3) * rows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
 }
 
+// The cache as TMA sees it: (element, token of the page, head, page) with
+// boxes of 64 elements and `run` tokens; run 0: it cannot be read that way.
+struct WideMaps {
+    CUtensorMap k, v;
+    int run;
+};
+
+__device__ __forceinline__ void tma_box(unsigned dst, const CUtensorMap *map, int x, int token, int head, int page, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(token), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // The loading warps of one kind (K with Q, or V): WARPS of them, of which this
 // is the w-th. A lane looks up the cells of every 32nd key of its warp's share.
 template <typename T, int HDP, int WARPS, bool KEYS>
-__device__ void load_tiles(const ptc_attn_args &a, int group, const int *pre, int u0, int u1, WideShared &sh, unsigned q_at, unsigned at, int w,
+__device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int run, int group, const int *pre, int u0, int u1, WideShared &sh, unsigned q_at, unsigned at, int w,
                            const Waiter &wait) {
     using S = WideShape<HDP>;
     constexpr int CH = HDP / 8, SHARE = WA_KEYS / WARPS, LOOKS = SHARE / 32;
@@ -206,8 +224,32 @@ __device__ void load_tiles(const ptc_attn_args &a, int group, const int *pre, in
             }
             over.issued(&sh.bar.q_full);
         }
+        // a lane's run of a tile: its page, looked up one tile ahead
+        auto look = [&](int j) {
+            const int t = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS + w * SHARE + lane * run;
+            return run && lane * run < SHARE && j < tiles && t < it.hi ? table[t / a.cache.page_size] : 0;
+        };
+        int page = look(0);
         for (int j = 0; j < tiles; j++, n++) {
-            const int t0 = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS + w * SHARE + lane;
+            const int s = n & 1, first = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS;
+            const int mine = page;
+            page = look(j + 1);
+            if (run && first >= it.lo && first + WA_KEYS <= it.hi && __all_sync(0xffffffffu, (unsigned)mine < (unsigned)a.cache.n_pages)) {
+                if (KEYS && lane < LOOKS) sh.bad[n & 3][w * LOOKS + lane] = 0;
+                if (n >= 2) wait(&empty[s], ((n >> 1) - 1) & 1);
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(&full[s], SHARE * HDP * 2);
+                else mbar_arrive(&full[s]);
+                if (lane * run < SHARE) {
+                    const int key = w * SHARE + lane * run, off = (first + key) % a.cache.page_size;
+#pragma unroll
+                    for (int b = 0; b < HDP / 64; b++)
+                        tma_box(at + s * S::KV + b * WA_KEYS * 128 + key * 128, map, b * 64, off, it.head, mine, &full[s]);
+                }
+                over.done<0>();
+                continue;
+            }
+            const int t0 = first + w * SHARE + lane;
             long long cell[LOOKS];
 #pragma unroll
             for (int g = 0; g < LOOKS; g++) {
@@ -222,8 +264,10 @@ __device__ void load_tiles(const ptc_attn_args &a, int group, const int *pre, in
                 const unsigned bad = __ballot_sync(0xffffffffu, want && cell[g] < 0);
                 if (KEYS && lane == 0) sh.bad[n & 3][w * LOOKS + g] = bad;
             }
-            const int s = n & 1;
-            if (n >= 2) wait(&empty[s], ((n >> 1) - 1) & 1);
+            if (n >= 2 && !__all_sync(0xffffffffu, mbar_try_wait(&empty[s], ((n >> 1) - 1) & 1))) {
+                over.done<0>();   // the stage is still read: meanwhile hand over what has landed
+                wait(&empty[s], ((n >> 1) - 1) & 1);
+            }
             __syncwarp();
 #pragma unroll
             for (int g = 0; g < LOOKS; g++)
@@ -242,7 +286,7 @@ __device__ void load_tiles(const ptc_attn_args &a, int group, const int *pre, in
 }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, int group) {
+__global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, const __grid_constant__ WideMaps maps, int group) {
     using S = WideShape<HDP>;
     extern __shared__ char wa_raw[];
     __shared__ WideShared sh;
@@ -283,9 +327,9 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, in
     const Waiter wait = {&sh.gave_up, a.err};
 
     if (warp >= 9 + WA_K_WARPS) {
-        load_tiles<T, HDP, WA_V_WARPS, false>(a, group, pre, u0, u1, sh, q_at, v_at, warp - 9 - WA_K_WARPS, wait);
+        load_tiles<T, HDP, WA_V_WARPS, false>(a, &maps.v, maps.run, group, pre, u0, u1, sh, q_at, v_at, warp - 9 - WA_K_WARPS, wait);
     } else if (warp >= 9) {
-        load_tiles<T, HDP, WA_K_WARPS, true>(a, group, pre, u0, u1, sh, q_at, k_at, warp - 9, wait);
+        load_tiles<T, HDP, WA_K_WARPS, true>(a, &maps.k, maps.run, group, pre, u0, u1, sh, q_at, k_at, warp - 9, wait);
     } else if (warp == 8) {
         // ---- products ----
         if (lane == 0) {
@@ -523,6 +567,34 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, in
     if (warp == 8) tm_free(tm, S::COLS);
 }
 
+// The tensor maps of a cache. Where a page's tokens do not come in runs of 8, or
+// the driver does not take the strides, run stays 0 and the copies serve.
+static WideMaps wide_maps(const ptc_paged_cache &c) {
+    WideMaps m;
+    memset(&m, 0, sizeof(m));
+    int run = 64;
+    while (c.page_size % run) run /= 2;
+    if (run < 8) return m;
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess || !fn) {
+        cudaGetLastError();
+        return m;
+    }
+    const auto encode = (decltype(&cuTensorMapEncodeTiled))fn;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv_heads, (cuuint64_t)c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.token_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)run, 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = c.dtype == PTC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int i = 0; i < 2; i++)
+        if (encode(i ? &m.v : &m.k, type, 4, i ? c.v : c.k, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return m;
+    m.run = run;
+    return m;
+}
+
 template <typename T, int HDP>
 static cudaError_t launch_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
     using S = WideShape<HDP>;
@@ -532,7 +604,7 @@ static cudaError_t launch_wide(const ptc_attn_args &a, int group, int n_sm, cuda
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const long long fit = (long long)(PTC_ATTN_WORKSPACE_BYTES - ATTN_FLAG_BYTES) / (2 * S::SLOT * (int)sizeof(float));
-    kernel<<<(unsigned)(n_sm < fit ? n_sm : fit), WA_THREADS, smem, s>>>(a, group);
+    kernel<<<(unsigned)(n_sm < fit ? n_sm : fit), WA_THREADS, smem, s>>>(a, wide_maps(a.cache), group);
     return cudaGetLastError();
 }
 
