@@ -9,8 +9,9 @@
 //                   tensor memory, running maximum and sum, probabilities back
 //                   to tensor memory as the A operand of the second product
 //   warp 8          one thread issues the products: S = Q K^T (128 x 128 per
-//                   tile) and O += P V, in an order in which each S follows
-//                   the product that read the P in the same place
+//                   tile) and O += P V, the latter in halves of 64 keys, as soon
+//                   as each half's probabilities are there, in an order in which
+//                   each S follows the products that read the P in the same place
 //   warps 9-10      Q and K tiles into shared memory, warp 11 V tiles, in the
 //                   128-byte swizzle that the tensor cores read: whole tiles by
 //                   TMA, a box per run of tokens that lie in one page (8 to 64),
@@ -28,14 +29,17 @@
 #include <limits.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "ptc_serve_attn.cuh"
 
 namespace ptc {
 
-constexpr int WA_ROWS = 256, WA_TILE = 128, WA_KEYS = 128;
+constexpr int WA_ROWS = 256, WA_TILE = 128, WA_KEYS = 128, WA_HALF = 64;
 constexpr int WA_THREADS = 12 * 32;
 constexpr int WA_K_WARPS = 2, WA_V_WARPS = 1;   // that load
 constexpr float WA_RISE = 8.f;
+constexpr int WA_POLY = 0;   // of four exponentials, those in multiply-adds
 
 // ---- tcgen05 ------------------------------------------------------------------
 
@@ -63,37 +67,59 @@ __device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, uint64_t b, un
         "r"(idesc), "r"((int)add)
         : "memory");
 }
-// 32 columns of this warp's 32 lanes. The values may be used after tm_wait_ld on them.
-__device__ __forceinline__ void tm_ld32(uint32_t (&r)[32], unsigned at) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
-        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(at));
+// Columns of this warp's 32 lanes. Loaded values may be used after tm_wait_ld on
+// them (the registers pass through it, so that no use moves before it).
+__device__ __forceinline__ void tm_ld16(uint32_t (&r)[16], unsigned at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
 }
-// (the registers pass through it, so that no use moves before it)
-__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
-                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
-                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tm_st32(unsigned at, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
-        "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+__device__ __forceinline__ void tm_st16(unsigned at, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, "
+                 "%9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                   "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tm_ld32(uint32_t (&r)[32], unsigned at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+                   "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+                   "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                   "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+                   "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 2^x for x <= 8 in fused multiply-adds (the special function unit does 16 a
+// clock and SM, and is what the softmax waits for): x = n + f, |f| <= 1/2, by
+// the cubic with the least largest error, 2^-13.7 relative -- the result is
+// rounded to 2^-9 or 2^-12.
+__device__ __forceinline__ float exp2_poly(float x) {
+    x = fmaxf(x, -126.f);
+    const float t = x + 12582912.f;   // 1.5 * 2^23: the sum's low bits are n
+    const float f = x - (t - 12582912.f);
+    const float p = fmaf(fmaf(fmaf(0.05517166f, f, 0.24261113f), f, 0.69326097f), f, 0.99992806f);
+    return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
+}
 
 // Shared-memory operand in the 128-byte swizzle: 16-bit elements in blocks of
 // 64 columns (128 bytes a row), 8 rows an atom of 1024 bytes.
@@ -113,7 +139,9 @@ __device__ __forceinline__ unsigned instruction(int n, bool b_mn) {
 // ---- the kernel -----------------------------------------------------------------
 
 struct WideBars {
-    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], done;
+    uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t s_full[2], p_full[2][2];      // by row tile; by row tile and half of the keys
+    uint64_t o_full[2], done;              // an item's last product into O; all products
 };
 
 struct WideShared {
@@ -313,7 +341,8 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
             mbar_init(&b.k_empty[i], 1);
             mbar_init(&b.v_empty[i], 1);
             mbar_init(&b.s_full[i], 1);
-            mbar_init(&b.p_full[i], WA_TILE);
+            mbar_init(&b.p_full[i][0], WA_TILE);
+            mbar_init(&b.p_full[i][1], WA_TILE);
             mbar_init(&b.o_full[i], 1);
         }
         sh.gave_up = 0;
@@ -334,7 +363,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         // ---- products ----
         if (lane == 0) {
             const unsigned id_s = instruction<T>(WA_KEYS, false), id_o = instruction<T>(HDP, true);
-            int n = 0, items = 0, pc[2] = {0, 0};
+            int n = 0, items = 0, p_phase[2] = {0, 0};   // K/V tiles that each row tile has had
             auto scores = [&](int t, int s) {   // S_t = Q_t K^T
 #pragma unroll
                 for (int k = 0; k < HDP / 16; k++) {
@@ -357,12 +386,15 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                     wait(&sh.bar.v_full[s], (n >> 1) & 1);
                     if (j + 1 < tiles) wait(&sh.bar.k_full[s ^ 1], ((n + 1) >> 1) & 1);
                     for (int t = 0; t < both; t++) {
-                        wait(&sh.bar.p_full[t], pc[t]++ & 1);
-                        tc_after_sync();
+                        for (int h = 0; h < 2; h++) {
+                            wait(&sh.bar.p_full[t][h], p_phase[t] & 1);
+                            tc_after_sync();
 #pragma unroll
-                        for (int k = 0; k < WA_KEYS / 16; k++)   // O_t += P_t V, 16 keys a step
-                            tc_mma_ts(tm + 2 * WA_KEYS + t * HDP, tm + t * WA_KEYS + k * 8, operand(v_at + s * S::KV + k * 2048, WA_KEYS * 128), id_o,
-                                      j > 0 || k > 0);
+                            for (int k = 0; k < WA_HALF / 16; k++)   // O_t += P_t V, 16 keys a step
+                                tc_mma_ts(tm + 2 * WA_KEYS + t * HDP, tm + t * WA_KEYS + h * (WA_HALF / 2) + k * 8,
+                                          operand(v_at + s * S::KV + (h * WA_HALF + k * 16) * 128, WA_KEYS * 128), id_o, j > 0 || h > 0 || k > 0);
+                        }
+                        p_phase[t]++;
                         if (j + 1 < tiles) scores(t, s ^ 1);
                         else tc_commit(&sh.bar.o_full[t]);
                     }
@@ -383,7 +415,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         const unsigned lanes = (unsigned)(warp & 3) << 21;   // this warp's 32 lanes of tensor memory
         const unsigned s_tm = tm + t * WA_KEYS + lanes, o_tm = tm + 2 * WA_KEYS + t * HDP + lanes;
         const float scale = a.scale * LOG2E;
-        int n = 0, sc = 0, oc = 0;
+        int n = 0, sc = 0, ic = 0;   // K/V tiles; those of this row tile; its items
         for (int u = u0; u < u1;) {
             const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
             const int seg0 = u - it.first, tiles = min(it.units - seg0, u1 - u), rows = it.i1 - it.i0;
@@ -399,83 +431,87 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                     wait(&sh.bar.s_full[t], sc & 1);
                     __syncwarp();   // (the accesses to tensor memory are the warp's)
                     tc_after_sync();
+                    uint32_t x[4][32];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) tm_ld32(x[q], s_tm + q * 32);
                     const unsigned *bad = sh.bad[(n + j) & 3];
                     const bool any_bad = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
                     const bool mask = any_bad || __any_sync(0xffffffffu, key0 + WA_KEYS > hi || key0 < lo);
-                    auto hide = [&](uint32_t(&r)[32], int q) {   // what this row does not see of columns 32 q on
-#pragma unroll
-                        for (int k = 0; k < 32; k++) {
-                            const int key = key0 + q * 32 + k;
-                            if (key >= hi || key < lo || (any_bad && (bad[q] >> k & 1))) r[k] = __float_as_uint(-INFINITY);
-                        }
-                    };
-                    uint32_t x[32], y[32];
                     float top = -INFINITY;
 #pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        tm_ld32(x, s_tm + q * 32);
-                        tm_ld32(y, s_tm + q * 32 + 32);
-                        tm_wait_ld(x);
-                        tm_wait_ld(y);
-                        if (mask) {
-                            hide(x, q);
-                            hide(y, q + 1);
-                        }
+                    for (int q = 0; q < 4; q++) {
+                        tm_wait_ld(x[q]);
+                        if (mask) {   // what this row does not see
 #pragma unroll
-                        for (int k = 0; k < 32; k++) top = fmaxf(top, fmaxf(__uint_as_float(x[k]), __uint_as_float(y[k])));
+                            for (int k = 0; k < 32; k++) {
+                                const int key = key0 + q * 32 + k;
+                                if (key >= hi || key < lo || (any_bad && (bad[q] >> k & 1))) x[q][k] = __float_as_uint(-INFINITY);
+                            }
+                        }
+                        float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            m0 = fmaxf(m0, fmaxf(__uint_as_float(x[q][k]), __uint_as_float(x[q][k + 1])));
+                            m1 = fmaxf(m1, fmaxf(__uint_as_float(x[q][k + 2]), __uint_as_float(x[q][k + 3])));
+                        }
+                        top = fmaxf(top, fmaxf(m0, m1));
                     }
                     top *= scale;
-                    const bool rise = top > m + WA_RISE || (m == -INFINITY && top > -INFINITY);
+                    const bool rise = top > m + WA_RISE;
                     if (j == 0) {
                         m = top;
                     } else if (__any_sync(0xffffffffu, rise)) {
-                        // (the S that was waited for follows the last product into O)
+                        // (the scores that were waited for follow the last product into O)
                         const float f = rise ? exp2f(m - top) : 1.f;
                         if (rise) m = top;
                         l *= f;
+#pragma unroll 1
+                        for (int d = 0; d < HDP; d += 16) {
+                            uint32_t o[16];
+                            tm_ld16(o, o_tm + d);
+                            tm_wait_ld(o);
 #pragma unroll
-                        for (int d = 0; d < HDP; d += 32) {
-                            tm_ld32(x, o_tm + d);
-                            tm_wait_ld(x);
-#pragma unroll
-                            for (int k = 0; k < 32; k++) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
-                            tm_st32(o_tm + d, x);
+                            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                            tm_st16(o_tm + d, o);
                         }
                         tm_wait_st();
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    // 32 probabilities, rounded to the type for the product with V (their sum is not);
+                    // exp2_poly has no zero, which what is masked has to become
+                    auto chunk = [&](int q, auto masked) {
+                        uint32_t p[16];
 #pragma unroll
-                    for (int q = 0; q < 4; q += 2) {
-                        tm_ld32(x, s_tm + q * 32);
-                        tm_ld32(y, s_tm + q * 32 + 32);
-                        tm_wait_ld(x);
-                        tm_wait_ld(y);
+                        for (int k = 0; k < 32; k += 4) {
+                            float e[4];
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; i4++) {
+                                e[i4] = fmaf(__uint_as_float(x[q][k + i4]), scale, -ref);
+                                e[i4] = masked.value || i4 < 4 - WA_POLY ? exp2_fast(e[i4]) : exp2_poly(e[i4]);
+                                sum[i4] += e[i4];
+                            }
+                            p[k / 2] = pack2(e[0], e[1], T());
+                            p[k / 2 + 1] = pack2(e[2], e[3], T());
+                        }
+                        tm_st16(s_tm + q * 16, p);
+                    };
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
                         if (mask) {
-                            hide(x, q);
-                            hide(y, q + 1);
+                            chunk(2 * h, std::true_type());
+                            chunk(2 * h + 1, std::true_type());
+                        } else {
+                            chunk(2 * h, std::false_type());
+                            chunk(2 * h + 1, std::false_type());
                         }
-                        // rounded to the type for the product with V (their sum is not)
-                        uint32_t p[32];
-#pragma unroll
-                        for (int k = 0; k < 32; k += 2) {
-                            const float e0 = exp2_fast(fmaf(__uint_as_float(x[k]), scale, -ref)), e1 = exp2_fast(fmaf(__uint_as_float(x[k + 1]), scale, -ref));
-                            const float e2 = exp2_fast(fmaf(__uint_as_float(y[k]), scale, -ref)), e3 = exp2_fast(fmaf(__uint_as_float(y[k + 1]), scale, -ref));
-                            sum[0] += e0;
-                            sum[1] += e1;
-                            sum[2] += e2;
-                            sum[3] += e3;
-                            p[k / 2] = pack2(e0, e1, T());
-                            p[16 + k / 2] = pack2(e2, e3, T());
-                        }
-                        tm_st32(s_tm + q * 16, p);
+                        tm_wait_st();
+                        tc_before_sync();
+                        mbar_arrive(&sh.bar.p_full[t][h]);
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tm_wait_st();
-                    tc_before_sync();
-                    mbar_arrive(&sh.bar.p_full[t]);
                 }
-                wait(&sh.bar.o_full[t], oc++ & 1);
+                wait(&sh.bar.o_full[t], ic++ & 1);
                 __syncwarp();
                 tc_after_sync();
             }
