@@ -39,7 +39,9 @@ constexpr int WA_ROWS = 256, WA_TILE = 128, WA_KEYS = 128, WA_HALF = 64;
 constexpr int WA_THREADS = 12 * 32;
 constexpr int WA_K_WARPS = 2, WA_V_WARPS = 1;   // that load
 constexpr float WA_RISE = 8.f;
-constexpr int WA_POLY = 0;   // of four exponentials, those in multiply-adds
+// Tensor memory, all 512 columns of it (so it begins at column 0).
+constexpr unsigned TM_S = 0, TM_O = 2 * WA_KEYS;
+constexpr int TM_COLS = 512;
 
 // ---- tcgen05 ------------------------------------------------------------------
 
@@ -54,6 +56,12 @@ __device__ __forceinline__ void tc_before_sync() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    unsigned yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes != 0;
 }
 __device__ __forceinline__ void tc_mma_ss(unsigned d, uint64_t a, uint64_t b, unsigned idesc, bool add) {
     asm volatile(
@@ -109,18 +117,6 @@ __device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 2^x for x <= 8 in fused multiply-adds (the special function unit does 16 a
-// clock and SM, and is what the softmax waits for): x = n + f, |f| <= 1/2, by
-// the cubic with the least largest error, 2^-13.7 relative -- the result is
-// rounded to 2^-9 or 2^-12.
-__device__ __forceinline__ float exp2_poly(float x) {
-    x = fmaxf(x, -126.f);
-    const float t = x + 12582912.f;   // 1.5 * 2^23: the sum's low bits are n
-    const float f = x - (t - 12582912.f);
-    const float p = fmaf(fmaf(fmaf(0.05517166f, f, 0.24261113f), f, 0.69326097f), f, 0.99992806f);
-    return __int_as_float(__float_as_int(p) + (__float_as_int(t) << 23));
-}
-
 // Shared-memory operand in the 128-byte swizzle: 16-bit elements in blocks of
 // 64 columns (128 bytes a row), 8 rows an atom of 1024 bytes.
 //   along K (rows are M or N): atoms `1024` apart
@@ -157,7 +153,6 @@ template <int HDP>
 struct WideShape {
     static constexpr int Q = WA_ROWS * HDP * 2, KV = WA_KEYS * HDP * 2;
     static constexpr int BYTES = Q + 4 * KV;                // Q, two K, two V
-    static constexpr int COLS = 512;                        // of tensor memory
     static constexpr int SLOT = WA_ROWS * (HDP + 2);        // floats of a workspace slot
 };
 
@@ -319,7 +314,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
     extern __shared__ char wa_raw[];
     __shared__ WideShared sh;
     char *wa_smem = wa_raw + (-smem_u32(wa_raw) & 1023);   // the swizzle is by address: whole atoms
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, heads = a.cache.n_kv_heads, hd = a.cache.head_dim;
+    const int tid = threadIdx.x, warp = tid >> 5, heads = a.cache.n_kv_heads, hd = a.cache.head_dim;
     const unsigned q_at = smem_u32(wa_smem), k_at = q_at + S::Q, v_at = k_at + 2 * S::KV;
     int *pre = (int *)(wa_smem + S::BYTES);
     unsigned *flags = (unsigned *)a.workspace;
@@ -348,11 +343,10 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         sh.gave_up = 0;
         mbar_init_fence();
     }
-    if (warp == 8) tm_alloc(&sh.tmem, S::COLS);
+    if (warp == 8) tm_alloc(&sh.tmem, TM_COLS);
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
-    const unsigned tm = sh.tmem;
     const Waiter wait = {&sh.gave_up, a.err};
 
     if (warp >= 9 + WA_K_WARPS) {
@@ -361,59 +355,90 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         load_tiles<T, HDP, WA_K_WARPS, true>(a, &maps.k, maps.run, group, pre, u0, u1, sh, q_at, k_at, warp - 9, wait);
     } else if (warp == 8) {
         // ---- products ----
-        if (lane == 0) {
-            const unsigned id_s = instruction<T>(WA_KEYS, false), id_o = instruction<T>(HDP, true);
-            int n = 0, items = 0, p_phase[2] = {0, 0};   // K/V tiles that each row tile has had
-            auto scores = [&](int t, int s) {   // S_t = Q_t K^T
+        // The warp stays together and one elected lane issues. Every operand is
+        // known before the loop (shared memory at its place, all of the tensor
+        // memory, the two stages as two copies of the code), so none has to be
+        // brought into the uniform registers that the instruction reads.
+        constexpr int IN_BLOCK = 4;   // steps of 16 columns in a swizzled block
+        const unsigned id_s = instruction<T>(WA_KEYS, false), id_o = instruction<T>(HDP, true);
+        auto scores = [&](auto t_, auto s_) {   // S_t = Q_t K^T
+            constexpr int t = t_.value, s = s_.value;
 #pragma unroll
-                for (int k = 0; k < HDP / 16; k++) {
-                    const unsigned off = (k >> 2) * WA_TILE * 128 + (k & 3) * 32;
-                    tc_mma_ss(tm + t * WA_KEYS, operand(q_at + t * (S::Q / 2) + off, 16), operand(k_at + s * S::KV + off, 16), id_s, k > 0);
-                }
-                tc_commit(&sh.bar.s_full[t]);
-            };
-            for (int u = u0; u < u1; items++) {
-                const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
-                const int tiles = min(it.units - (u - it.first), u1 - u), both = it.i1 - it.i0 > WA_TILE ? 2 : 1;
-                wait(&sh.bar.q_full, items & 1);
-                wait(&sh.bar.k_full[n & 1], (n >> 1) & 1);
-                tc_after_sync();
-                for (int t = 0; t < both; t++) scores(t, n & 1);
-                tc_commit(&sh.bar.k_empty[n & 1]);
-                if (tiles == 1) tc_commit(&sh.bar.q_empty);
-                for (int j = 0; j < tiles; j++, n++) {
-                    const int s = n & 1;
-                    wait(&sh.bar.v_full[s], (n >> 1) & 1);
-                    if (j + 1 < tiles) wait(&sh.bar.k_full[s ^ 1], ((n + 1) >> 1) & 1);
-                    for (int t = 0; t < both; t++) {
-                        for (int h = 0; h < 2; h++) {
-                            wait(&sh.bar.p_full[t][h], p_phase[t] & 1);
-                            tc_after_sync();
-#pragma unroll
-                            for (int k = 0; k < WA_HALF / 16; k++)   // O_t += P_t V, 16 keys a step
-                                tc_mma_ts(tm + 2 * WA_KEYS + t * HDP, tm + t * WA_KEYS + h * (WA_HALF / 2) + k * 8,
-                                          operand(v_at + s * S::KV + (h * WA_HALF + k * 16) * 128, WA_KEYS * 128), id_o, j > 0 || h > 0 || k > 0);
-                        }
-                        p_phase[t]++;
-                        if (j + 1 < tiles) scores(t, s ^ 1);
-                        else tc_commit(&sh.bar.o_full[t]);
-                    }
-                    tc_commit(&sh.bar.v_empty[s]);
-                    if (j + 1 < tiles) tc_commit(&sh.bar.k_empty[s ^ 1]);
-                    if (j + 2 == tiles) tc_commit(&sh.bar.q_empty);
-                }
-                u += tiles;
+            for (int k = 0; k < HDP / 16; k++) {
+                const unsigned off = (k / IN_BLOCK) * WA_TILE * 128 + (k % IN_BLOCK) * 32;
+                tc_mma_ss(TM_S + t * WA_KEYS, operand(q_at + t * (S::Q / 2) + off, 16), operand(k_at + s * S::KV + off, 16), id_s, k > 0);
             }
-            // (every product has been waited for, unless a wait has given up)
-            tc_commit(&sh.bar.done);
-            wait(&sh.bar.done, 0);
+            tc_commit(&sh.bar.s_full[t]);
+        };
+        auto values = [&](auto t_, auto s_, auto h_, bool add) {   // O_t += P_t V of half h of the keys, 16 a step
+            constexpr int t = t_.value, s = s_.value, h = h_.value;
+#pragma unroll
+            for (int k = 0; k < WA_HALF / 16; k++)
+                tc_mma_ts(TM_O + t * HDP, TM_S + t * WA_KEYS + h * (WA_HALF / 2) + k * 8,
+                          operand(v_at + s * S::KV + (h * WA_HALF + k * 16) * 128, WA_KEYS * 128), id_o, add || h > 0 || k > 0);
+        };
+        int n = 0, items = 0, phase[2] = {0, 0};   // K/V tiles, items, K/V tiles of each row tile
+        // the products of one K/V tile, stage s, and the scores of the next
+        auto step = [&](auto s_, bool both, bool add, bool more, bool done) {
+            constexpr int s = s_.value;
+            typedef std::integral_constant<int, 1 - s> Other;
+            wait(&sh.bar.v_full[s], (n >> 1) & 1);
+            if (more) wait(&sh.bar.k_full[1 - s], ((n + 1) >> 1) & 1);
+            auto tile = [&](auto t_) {
+                constexpr int t = t_.value;
+                wait(&sh.bar.p_full[t][0], phase[t] & 1);
+                tc_after_sync();
+                if (elect_one()) values(t_, s_, std::integral_constant<int, 0>(), add);
+                wait(&sh.bar.p_full[t][1], phase[t] & 1);
+                tc_after_sync();
+                if (elect_one()) {
+                    values(t_, s_, std::integral_constant<int, 1>(), true);
+                    if (more) scores(t_, Other());
+                    else tc_commit(&sh.bar.o_full[t]);
+                }
+                phase[t]++;
+            };
+            tile(std::integral_constant<int, 0>());
+            if (both) tile(std::integral_constant<int, 1>());
+            if (elect_one()) {
+                tc_commit(&sh.bar.v_empty[s]);
+                if (more) tc_commit(&sh.bar.k_empty[1 - s]);
+                if (done) tc_commit(&sh.bar.q_empty);
+            }
+        };
+        auto first = [&](auto s_, bool both, bool done) {
+            constexpr int s = s_.value;
+            if (elect_one()) {
+                scores(std::integral_constant<int, 0>(), s_);
+                if (both) scores(std::integral_constant<int, 1>(), s_);
+                tc_commit(&sh.bar.k_empty[s]);
+                if (done) tc_commit(&sh.bar.q_empty);
+            }
+        };
+        for (int u = u0; u < u1; items++) {
+            const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
+            const int tiles = min(it.units - (u - it.first), u1 - u);
+            const bool both = it.i1 - it.i0 > WA_TILE;
+            wait(&sh.bar.q_full, items & 1);
+            wait(&sh.bar.k_full[n & 1], (n >> 1) & 1);
+            tc_after_sync();
+            if (n & 1) first(std::integral_constant<int, 1>(), both, tiles == 1);
+            else first(std::integral_constant<int, 0>(), both, tiles == 1);
+            for (int j = 0; j < tiles; j++, n++) {
+                if (n & 1) step(std::integral_constant<int, 1>(), both, j > 0, j + 1 < tiles, j + 2 == tiles);
+                else step(std::integral_constant<int, 0>(), both, j > 0, j + 1 < tiles, j + 2 == tiles);
+            }
+            u += tiles;
         }
+        // (every product has been waited for, unless a wait has given up)
+        if (elect_one()) tc_commit(&sh.bar.done);
+        wait(&sh.bar.done, 0);
         __syncwarp();
     } else {
         // ---- softmax ----
         const int t = warp >> 2, row = tid & 127;
         const unsigned lanes = (unsigned)(warp & 3) << 21;   // this warp's 32 lanes of tensor memory
-        const unsigned s_tm = tm + t * WA_KEYS + lanes, o_tm = tm + 2 * WA_KEYS + t * HDP + lanes;
+        const unsigned s_tm = TM_S + t * WA_KEYS + lanes, o_tm = TM_O + t * HDP + lanes;
         const float scale = a.scale * LOG2E;
         int n = 0, sc = 0, ic = 0;   // K/V tiles; those of this row tile; its items
         for (int u = u0; u < u1;) {
@@ -478,32 +503,24 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    // 32 probabilities, rounded to the type for the product with V (their sum is not);
-                    // exp2_poly has no zero, which what is masked has to become
-                    auto chunk = [&](int q, auto masked) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            float e[4];
-#pragma unroll
-                            for (int i4 = 0; i4 < 4; i4++) {
-                                e[i4] = fmaf(__uint_as_float(x[q][k + i4]), scale, -ref);
-                                e[i4] = masked.value || i4 < 4 - WA_POLY ? exp2_fast(e[i4]) : exp2_poly(e[i4]);
-                                sum[i4] += e[i4];
-                            }
-                            p[k / 2] = pack2(e[0], e[1], T());
-                            p[k / 2 + 1] = pack2(e[2], e[3], T());
-                        }
-                        tm_st16(s_tm + q * 16, p);
-                    };
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (mask) {
-                            chunk(2 * h, std::true_type());
-                            chunk(2 * h + 1, std::true_type());
-                        } else {
-                            chunk(2 * h, std::false_type());
-                            chunk(2 * h + 1, std::false_type());
+#pragma unroll
+                        for (int q = 2 * h; q < 2 * h + 2; q++) {
+                            // rounded to the type for the product with V (their sum is not)
+                            uint32_t p[16];
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) {
+                                float e[4];
+#pragma unroll
+                                for (int i4 = 0; i4 < 4; i4++) {
+                                    e[i4] = exp2_fast(fmaf(__uint_as_float(x[q][k + i4]), scale, -ref));
+                                    sum[i4] += e[i4];
+                                }
+                                p[k / 2] = pack2(e[0], e[1], T());
+                                p[k / 2 + 1] = pack2(e[2], e[3], T());
+                            }
+                            tm_st16(s_tm + q * 16, p);
                         }
                         tm_wait_st();
                         tc_before_sync();
@@ -600,7 +617,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
-    if (warp == 8) tm_free(tm, S::COLS);
+    if (warp == 8) tm_free(TM_S, TM_COLS);
 }
 
 // The tensor maps of a cache. Where a page's tokens do not come in runs of 8, or
