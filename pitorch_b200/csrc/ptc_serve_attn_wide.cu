@@ -2,16 +2,18 @@
 // (include/ptc_serve.h): the kernel for many rows per K/V head, 16-bit types.
 //
 // One CTA per SM on tcgen05 tensor cores. An item has 256 rows, as two tiles
-// of 128 that share every K/V tile of 128 keys and take turns: while one
-// tile's scores become probabilities, the tensor cores work for the other.
+// of 128 that share every K/V tile of 128 keys. A row tile's keys are taken in
+// halves of 64, so that the scores of one half are made while the other half's
+// become probabilities: the softmax takes as long as the products, and neither
+// may wait for the other. (With 128 keys at a time, which tensor memory holds
+// once beside the outputs, a row tile's softmax and products alternate.)
 //
 //   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per row: scores from
 //                   tensor memory, running maximum and sum, probabilities back
 //                   to tensor memory as the A operand of the second product
-//   warp 8          one thread issues the products: S = Q K^T (128 x 128 per
-//                   tile) and O += P V, the latter in halves of 64 keys, as soon
-//                   as each half's probabilities are there, in an order in which
-//                   each S follows the products that read the P in the same place
+//   warp 8          one lane issues the products: S = Q K^T (128 x 64 per tile and
+//                   half) and O += P V, in an order in which each S follows the
+//                   product that read the P in the same place
 //   warps 9-10      Q and K tiles into shared memory, warp 11 V tiles, in the
 //                   128-byte swizzle that the tensor cores read: whole tiles by
 //                   TMA, a box per run of tokens that lie in one page (8 to 64),
@@ -21,7 +23,7 @@
 // Twelve warps are three to a scheduler, which leaves a thread 168 registers;
 // a thirteenth would leave 128.
 //
-// Tensor memory: S0 | S1 | O0 | O1; P takes the place of the first half of its
+// Tensor memory: S0 | S1 | O0 | O1; the P of a half takes the place of its
 // S. The running maximum is replaced, and O rescaled, only when it rises by
 // more than 2^8 (probabilities and sums are relative to the same value, so
 // nothing is lost: they stay below 2^8 and 2^8 times the keys).
@@ -136,8 +138,8 @@ __device__ __forceinline__ unsigned instruction(int n, bool b_mn) {
 
 struct WideBars {
     uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2], p_full[2][2];      // by row tile; by row tile and half of the keys
-    uint64_t o_full[2], done;              // an item's last product into O; all products
+    uint64_t s_full[2][2], p_full[2][2];   // by row tile and half of the keys
+    uint64_t o_done[2], o_full[2], done;   // a product into a tile's O; an item's last one; all products
 };
 
 struct WideShared {
@@ -335,9 +337,11 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
             mbar_init(&b.v_full[i], WA_V_WARPS * 32);
             mbar_init(&b.k_empty[i], 1);
             mbar_init(&b.v_empty[i], 1);
-            mbar_init(&b.s_full[i], 1);
-            mbar_init(&b.p_full[i][0], WA_TILE);
-            mbar_init(&b.p_full[i][1], WA_TILE);
+            for (int h = 0; h < 2; h++) {
+                mbar_init(&b.s_full[i][h], 1);
+                mbar_init(&b.p_full[i][h], WA_TILE);
+            }
+            mbar_init(&b.o_done[i], 1);
             mbar_init(&b.o_full[i], 1);
         }
         sh.gave_up = 0;
@@ -360,46 +364,49 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         // memory, the two stages as two copies of the code), so none has to be
         // brought into the uniform registers that the instruction reads.
         constexpr int IN_BLOCK = 4;   // steps of 16 columns in a swizzled block
-        const unsigned id_s = instruction<T>(WA_KEYS, false), id_o = instruction<T>(HDP, true);
-        auto scores = [&](auto t_, auto s_) {   // S_t = Q_t K^T
-            constexpr int t = t_.value, s = s_.value;
+        const unsigned id_s = instruction<T>(WA_HALF, false), id_o = instruction<T>(HDP, true);
+        typedef std::integral_constant<int, 0> Zero;
+        typedef std::integral_constant<int, 1> One;
+        auto scores = [&](auto t_, auto h_, auto s_) {   // S_t = Q_t K^T of half h of the keys
+            constexpr int t = t_.value, h = h_.value, s = s_.value;
 #pragma unroll
             for (int k = 0; k < HDP / 16; k++) {
                 const unsigned off = (k / IN_BLOCK) * WA_TILE * 128 + (k % IN_BLOCK) * 32;
-                tc_mma_ss(TM_S + t * WA_KEYS, operand(q_at + t * (S::Q / 2) + off, 16), operand(k_at + s * S::KV + off, 16), id_s, k > 0);
+                tc_mma_ss(TM_S + t * WA_KEYS + h * WA_HALF, operand(q_at + t * (S::Q / 2) + off, 16),
+                          operand(k_at + s * S::KV + h * WA_HALF * 128 + off, 16), id_s, k > 0);
             }
-            tc_commit(&sh.bar.s_full[t]);
+            tc_commit(&sh.bar.s_full[t][h]);
         };
-        auto values = [&](auto t_, auto s_, auto h_, bool add) {   // O_t += P_t V of half h of the keys, 16 a step
-            constexpr int t = t_.value, s = s_.value, h = h_.value;
+        auto values = [&](auto t_, auto h_, auto s_, bool add) {   // O_t += P_t V of half h of the keys, 16 a step
+            constexpr int t = t_.value, h = h_.value, s = s_.value;
 #pragma unroll
             for (int k = 0; k < WA_HALF / 16; k++)
-                tc_mma_ts(TM_O + t * HDP, TM_S + t * WA_KEYS + h * (WA_HALF / 2) + k * 8,
-                          operand(v_at + s * S::KV + (h * WA_HALF + k * 16) * 128, WA_KEYS * 128), id_o, add || h > 0 || k > 0);
+                tc_mma_ts(TM_O + t * HDP, TM_S + t * WA_KEYS + h * WA_HALF + k * 8, operand(v_at + s * S::KV + (h * WA_HALF + k * 16) * 128, WA_KEYS * 128),
+                          id_o, add || h > 0 || k > 0);
+            tc_commit(&sh.bar.o_done[t]);
         };
         int n = 0, items = 0, phase[2] = {0, 0};   // K/V tiles, items, K/V tiles of each row tile
         // the products of one K/V tile, stage s, and the scores of the next
         auto step = [&](auto s_, bool both, bool add, bool more, bool done) {
             constexpr int s = s_.value;
-            typedef std::integral_constant<int, 1 - s> Other;
             wait(&sh.bar.v_full[s], (n >> 1) & 1);
             if (more) wait(&sh.bar.k_full[1 - s], ((n + 1) >> 1) & 1);
-            auto tile = [&](auto t_) {
-                constexpr int t = t_.value;
-                wait(&sh.bar.p_full[t][0], phase[t] & 1);
-                tc_after_sync();
-                if (elect_one()) values(t_, s_, std::integral_constant<int, 0>(), add);
-                wait(&sh.bar.p_full[t][1], phase[t] & 1);
+            auto part = [&](auto t_, auto h_) {
+                constexpr int t = t_.value, h = h_.value;
+                wait(&sh.bar.p_full[t][h], phase[t] & 1);
                 tc_after_sync();
                 if (elect_one()) {
-                    values(t_, s_, std::integral_constant<int, 1>(), true);
-                    if (more) scores(t_, Other());
-                    else tc_commit(&sh.bar.o_full[t]);
+                    values(t_, h_, s_, add);
+                    if (more) scores(t_, h_, std::integral_constant<int, 1 - s>());
+                    else if (h == 1) tc_commit(&sh.bar.o_full[t]);
                 }
-                phase[t]++;
             };
-            tile(std::integral_constant<int, 0>());
-            if (both) tile(std::integral_constant<int, 1>());
+            part(Zero(), Zero());
+            if (both) part(One(), Zero());
+            part(Zero(), One());
+            if (both) part(One(), One());
+            phase[0]++;
+            phase[1] += both;
             if (elect_one()) {
                 tc_commit(&sh.bar.v_empty[s]);
                 if (more) tc_commit(&sh.bar.k_empty[1 - s]);
@@ -409,8 +416,10 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         auto first = [&](auto s_, bool both, bool done) {
             constexpr int s = s_.value;
             if (elect_one()) {
-                scores(std::integral_constant<int, 0>(), s_);
-                if (both) scores(std::integral_constant<int, 1>(), s_);
+                scores(Zero(), Zero(), s_);
+                if (both) scores(One(), Zero(), s_);
+                scores(Zero(), One(), s_);
+                if (both) scores(One(), One(), s_);
                 tc_commit(&sh.bar.k_empty[s]);
                 if (done) tc_commit(&sh.bar.q_empty);
             }
@@ -422,11 +431,11 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
             wait(&sh.bar.q_full, items & 1);
             wait(&sh.bar.k_full[n & 1], (n >> 1) & 1);
             tc_after_sync();
-            if (n & 1) first(std::integral_constant<int, 1>(), both, tiles == 1);
-            else first(std::integral_constant<int, 0>(), both, tiles == 1);
+            if (n & 1) first(One(), both, tiles == 1);
+            else first(Zero(), both, tiles == 1);
             for (int j = 0; j < tiles; j++, n++) {
-                if (n & 1) step(std::integral_constant<int, 1>(), both, j > 0, j + 1 < tiles, j + 2 == tiles);
-                else step(std::integral_constant<int, 0>(), both, j > 0, j + 1 < tiles, j + 2 == tiles);
+                if (n & 1) step(One(), both, j > 0, j + 1 < tiles, j + 2 == tiles);
+                else step(Zero(), both, j > 0, j + 1 < tiles, j + 2 == tiles);
             }
             u += tiles;
         }
@@ -440,7 +449,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
         const unsigned lanes = (unsigned)(warp & 3) << 21;   // this warp's 32 lanes of tensor memory
         const unsigned s_tm = TM_S + t * WA_KEYS + lanes, o_tm = TM_O + t * HDP + lanes;
         const float scale = a.scale * LOG2E;
-        int n = 0, sc = 0, ic = 0;   // K/V tiles; those of this row tile; its items
+        int n = 0, sc = 0, oc = 0, ic = 0;   // K/V tiles; those of this row tile, products into its O, its items
         for (int u = u0; u < u1;) {
             const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
             const int seg0 = u - it.first, tiles = min(it.units - seg0, u1 - u), rows = it.i1 - it.i0;
@@ -448,65 +457,68 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
             const int i = it.i0 + t * WA_TILE + row, tok = i / group;
             const bool real = i < it.i1;
             // rows that are not there see everything: their zeros need no masking
-            const int pos = it.s.pos0 + tok, hi = real ? min(pos + 1, it.s.cap) : INT_MAX, lo = real && a.window > 0 ? pos - a.window + 1 : INT_MIN;
+            const int pos = it.s.pos0 + tok, hi = real ? min(pos + 1, it.s.cap) : INT_MAX, lo = real && a.window > 0 ? pos - a.window + 1 : 0;
             float m = -INFINITY, l = 0.f;   // the reference of the probabilities, and their sum
             if (active) {
                 for (int j = 0; j < tiles; j++, sc++) {
-                    const int key0 = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS;
-                    wait(&sh.bar.s_full[t], sc & 1);
-                    __syncwarp();   // (the accesses to tensor memory are the warp's)
-                    tc_after_sync();
-                    uint32_t x[4][32];
+#pragma unroll 1   // (one copy: two do not stay in the instruction cache)
+                    for (int h = 0; h < 2; h++) {
+                        const int key0 = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS + h * WA_HALF;
+                        wait(&sh.bar.s_full[t][h], sc & 1);
+                        __syncwarp();   // (the accesses to tensor memory are the warp's)
+                        tc_after_sync();
+                        uint32_t x[2][32];
+                        tm_ld32(x[0], s_tm + h * WA_HALF);
+                        tm_ld32(x[1], s_tm + h * WA_HALF + 32);
+                        const unsigned *bad = &sh.bad[(n + j) & 3][2 * h];
+                        const bool mask = (bad[0] | bad[1]) != 0 || __any_sync(0xffffffffu, key0 + WA_HALF > hi || key0 < lo);
+                        float top = -INFINITY;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) tm_ld32(x[q], s_tm + q * 32);
-                    const unsigned *bad = sh.bad[(n + j) & 3];
-                    const bool any_bad = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
-                    const bool mask = any_bad || __any_sync(0xffffffffu, key0 + WA_KEYS > hi || key0 < lo);
-                    float top = -INFINITY;
+                        for (int q = 0; q < 2; q++) {
+                            tm_wait_ld(x[q]);
+                            if (mask) {   // what this row does not see: a bit per key
+                                const int from = max(0, lo - key0 - q * 32), to = hi - key0 - q * 32;
+                                unsigned see = to >= 32 ? ~0u : to > 0 ? (1u << to) - 1 : 0;
+                                see &= from >= 32 ? 0 : ~0u << from;
+                                see &= ~bad[q];
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        tm_wait_ld(x[q]);
-                        if (mask) {   // what this row does not see
+                                for (int k = 0; k < 32; k++)
+                                    if (!(see >> k & 1)) x[q][k] = __float_as_uint(-INFINITY);
+                            }
+                            float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-                            for (int k = 0; k < 32; k++) {
-                                const int key = key0 + q * 32 + k;
-                                if (key >= hi || key < lo || (any_bad && (bad[q] >> k & 1))) x[q][k] = __float_as_uint(-INFINITY);
+                            for (int k = 0; k < 32; k += 4) {
+                                m0 = fmaxf(m0, fmaxf(__uint_as_float(x[q][k]), __uint_as_float(x[q][k + 1])));
+                                m1 = fmaxf(m1, fmaxf(__uint_as_float(x[q][k + 2]), __uint_as_float(x[q][k + 3])));
+                            }
+                            top = fmaxf(top, fmaxf(m0, m1));
+                        }
+                        top *= scale;
+                        const bool rise = top > m + WA_RISE;
+                        if (j == 0 && h == 0) {
+                            m = top;
+                        } else if (__any_sync(0xffffffffu, rise)) {
+                            // (all products but the last one into this O were done when these scores were)
+                            wait(&sh.bar.o_done[t], (oc - 1) & 1);
+                            __syncwarp();
+                            tc_after_sync();
+                            const float f = rise ? exp2f(m - top) : 1.f;
+                            if (rise) m = top;
+                            l *= f;
+#pragma unroll 1
+                            for (int d = 0; d < HDP; d += 16) {
+                                uint32_t o[16];
+                                tm_ld16(o, o_tm + d);
+                                tm_wait_ld(o);
+#pragma unroll
+                                for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tm_st16(o_tm + d, o);
                             }
                         }
-                        float m0 = -INFINITY, m1 = -INFINITY;
+                        const float ref = m == -INFINITY ? 0.f : m;
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int k = 0; k < 32; k += 4) {
-                            m0 = fmaxf(m0, fmaxf(__uint_as_float(x[q][k]), __uint_as_float(x[q][k + 1])));
-                            m1 = fmaxf(m1, fmaxf(__uint_as_float(x[q][k + 2]), __uint_as_float(x[q][k + 3])));
-                        }
-                        top = fmaxf(top, fmaxf(m0, m1));
-                    }
-                    top *= scale;
-                    const bool rise = top > m + WA_RISE;
-                    if (j == 0) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, rise)) {
-                        // (the scores that were waited for follow the last product into O)
-                        const float f = rise ? exp2f(m - top) : 1.f;
-                        if (rise) m = top;
-                        l *= f;
-#pragma unroll 1
-                        for (int d = 0; d < HDP; d += 16) {
-                            uint32_t o[16];
-                            tm_ld16(o, o_tm + d);
-                            tm_wait_ld(o);
-#pragma unroll
-                            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                            tm_st16(o_tm + d, o);
-                        }
-                        tm_wait_st();
-                    }
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-#pragma unroll
-                        for (int q = 2 * h; q < 2 * h + 2; q++) {
+                        for (int q = 0; q < 2; q++) {
                             // rounded to the type for the product with V (their sum is not)
                             uint32_t p[16];
 #pragma unroll
@@ -520,13 +532,14 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                                 p[k / 2] = pack2(e[0], e[1], T());
                                 p[k / 2 + 1] = pack2(e[2], e[3], T());
                             }
-                            tm_st16(s_tm + q * 16, p);
+                            tm_st16(s_tm + h * WA_HALF + q * 16, p);
                         }
                         tm_wait_st();
                         tc_before_sync();
                         mbar_arrive(&sh.bar.p_full[t][h]);
+                        oc++;
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
                 wait(&sh.bar.o_full[t], ic++ & 1);
                 __syncwarp();
