@@ -296,7 +296,7 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
             __syncwarp();
 #pragma unroll
             for (int g = 0; g < LOOKS; g++)
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < CH; i++) {
                     const int x = i * 32 + lane, k = x / CH, ch = x % CH;
                     const long long c = __shfl_sync(0xffffffffu, cell[g], k);
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                 const float inv = l > 0.f ? 1.f / l : 0.f;
                 T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + i - tok * group) * hd;
                 float *part = slot + (t * WA_TILE + row) * HDP;
-#pragma unroll
+#pragma unroll 1
                 for (int d = 0; d < HDP; d += 32) {
                     uint32_t x[32];
                     tm_ld32(x, o_tm + d);
