@@ -15,11 +15,10 @@
 //                   half) and O += P V, in an order in which each S follows the
 //                   product that read the P in the same place
 //   warps 9-10      Q and K tiles into shared memory, warp 11 V tiles, in the
-//                   128-byte swizzle that the tensor cores read: whole tiles by
-//                   TMA, a box per run of tokens that lie in one page (8 to 64),
-//                   what ends inside a tile by 16-byte asynchronous copies with
-//                   zeros behind it, and so do page sizes that are no multiple
-//                   of 8
+//                   128-byte swizzle that the tensor cores read: by TMA, a box
+//                   for each run of tokens that lie in one page (8 to 64); by
+//                   16-byte asynchronous copies where a run ends behind the last
+//                   position, and where page sizes are no multiple of 8
 // Twelve warps are three to a scheduler, which leaves a thread 168 registers;
 // a thirteenth would leave 128.
 //
@@ -118,6 +117,19 @@ __device__ __forceinline__ void tm_wait_ld(uint32_t (&r)[32]) {
                  : "memory");
 }
 __device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two 32-bit operations in one instruction: (a, b) = (x, y) * s + t, (a, b) += (x, y).
+__device__ __forceinline__ void fma_pair(float &a, float &b, float x, float y, float s, float t) {
+    asm("{\n .reg .b64 u, v, w;\n mov.b64 u, {%2, %3};\n mov.b64 v, {%4, %4};\n mov.b64 w, {%5, %5};\n fma.rn.f32x2 u, u, v, w;\n"
+        " mov.b64 {%0, %1}, u;\n}"
+        : "=f"(a), "=f"(b)
+        : "f"(x), "f"(y), "f"(s), "f"(t));
+}
+__device__ __forceinline__ void add_pair(float &a, float &b, float x, float y) {
+    asm("{\n .reg .b64 u, v;\n mov.b64 u, {%0, %1};\n mov.b64 v, {%2, %3};\n add.rn.f32x2 u, u, v;\n mov.b64 {%0, %1}, u;\n}"
+        : "+f"(a), "+f"(b)
+        : "f"(x), "f"(y));
+}
 
 // Shared-memory operand in the 128-byte swizzle: 16-bit elements in blocks of
 // 64 columns (128 bytes a row), 8 rows an atom of 1024 bytes.
@@ -249,29 +261,86 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
             }
             over.issued(&sh.bar.q_full);
         }
-        // a lane's run of a tile: its page, looked up one tile ahead
+        // a lane's run of tokens of a tile: its page, looked up one tile ahead
+        const int key = w * SHARE + lane * run;
+        const bool runs = run && lane * run < SHARE;
         auto look = [&](int j) {
-            const int t = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS + w * SHARE + lane * run;
-            return run && lane * run < SHARE && j < tiles && t < it.hi ? table[t / a.cache.page_size] : 0;
+            const int t = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS + key;
+            return runs && j < tiles && t < it.hi && t + run > it.lo ? table[t / a.cache.page_size] : -1;
         };
         int page = look(0);
         for (int j = 0; j < tiles; j++, n++) {
-            const int s = n & 1, first = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS;
-            const int mine = page;
+            const int s = n & 1, first = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS, mine = page;
+            const unsigned stage = at + s * S::KV;
             page = look(j + 1);
-            if (run && first >= it.lo && first + WA_KEYS <= it.hi && __all_sync(0xffffffffu, (unsigned)mine < (unsigned)a.cache.n_pages)) {
+            if (run && first >= it.lo && first + WA_KEYS <= it.hi && __all_sync(0xffffffffu, !runs || (unsigned)mine < (unsigned)a.cache.n_pages)) {
+                // a whole tile
                 if (KEYS && lane < LOOKS) sh.bad[n & 3][w * LOOKS + lane] = 0;
                 if (n >= 2) wait(&empty[s], ((n >> 1) - 1) & 1);
                 __syncwarp();
                 if (lane == 0) mbar_expect_tx(&full[s], SHARE * HDP * 2);
                 else mbar_arrive(&full[s]);
-                if (lane * run < SHARE) {
-                    const int key = w * SHARE + lane * run, off = (first + key) % a.cache.page_size;
+                if (runs)
 #pragma unroll
                     for (int b = 0; b < HDP / 64; b++)
-                        tma_box(at + s * S::KV + b * WA_KEYS * 128 + key * 128, map, b * 64, off, it.head, mine, &full[s]);
-                }
+                        tma_box(stage + b * WA_KEYS * 128 + key * 128, map, b * 64, (first + key) % a.cache.page_size, it.head, mine, &full[s]);
                 over.done<0>();
+                continue;
+            }
+            if (run) {
+                // Whole runs by TMA, from the first that is seen on. A run that ends behind the last position is
+                // copied with zeros there, as what lies there may be anything, and V's other runs become zeros
+                // (the scores of K's are masked, whatever the stage holds).
+                const int t = first + key;
+                const bool seen = runs && t < it.hi && t + run > it.lo, there = (unsigned)mine < (unsigned)a.cache.n_pages;
+                const bool whole = seen && there && t + run <= it.hi;
+                if (KEYS) {
+                    if (lane < LOOKS) sh.bad[n & 3][w * LOOKS + lane] = 0;
+                    __syncwarp();
+                }
+                if (seen && !there) {
+                    serve_err(a.err, PTC_SERVE_ERR_INDEX);
+                    if (KEYS)
+                        for (int b = 0; b < run; b += 32) atomicOr(&sh.bad[n & 3][(key + b) >> 5], (run < 32 ? (1u << run) - 1 : ~0u) << (key & 31));
+                }
+                const int edge = __ffs(__ballot_sync(0xffffffffu, seen && there && !whole)) - 1;   // the lane of a run that ends inside
+                const unsigned boxes = __popc(__ballot_sync(0xffffffffu, whole));
+                if (n >= 2) {
+                    if (!__all_sync(0xffffffffu, mbar_try_wait(&empty[s], ((n >> 1) - 1) & 1))) over.done<0>();
+                    wait(&empty[s], ((n >> 1) - 1) & 1);
+                }
+                __syncwarp();
+                if (!KEYS) {
+                    unsigned none = __ballot_sync(0xffffffffu, runs && !(seen && there));
+                    if (none) {
+                        for (; none; none &= none - 1)
+                            for (int x = lane; x < run * CH; x += 32) {
+                                const int k = (__ffs(none) - 1) * run + x / CH;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + swizzled(WA_KEYS, k, x % CH)), "r"(0) : "memory");
+                            }
+                        fence_proxy_async_smem();
+                    }
+                }
+                if (lane == 0) asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[s])), "r"(boxes * run * HDP * 2) : "memory");
+                __syncwarp();
+                if (whole)
+#pragma unroll
+                    for (int b = 0; b < HDP / 64; b++)
+                        tma_box(stage + b * WA_KEYS * 128 + key * 128, map, b * 64, t % a.cache.page_size, it.head, mine, &full[s]);
+                if (edge >= 0) {
+                    const int p = __shfl_sync(0xffffffffu, mine, edge), k0 = w * SHARE + edge * run, te = first + k0;
+                    const long long cell = attn_cell(a, p, te % a.cache.page_size);
+#pragma unroll 4
+                    for (int x = lane; x < run * CH; x += 32) {
+                        const int k = x / CH, ch = x % CH;
+                        const bool real = te + k < it.hi && ch * 8 < hd;
+                        cp16_or_zero(stage + swizzled(WA_KEYS, k0 + k, ch), from + (real ? cell + k * a.cache.token_stride + head + ch * 8 : 0), real);
+                    }
+                    over.issued(&full[s]);
+                } else {
+                    over.done<0>();
+                    mbar_arrive(&full[s]);
+                }
                 continue;
             }
             const int t0 = first + w * SHARE + lane;
@@ -301,7 +370,7 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
                     const int x = i * 32 + lane, k = x / CH, ch = x % CH;
                     const long long c = __shfl_sync(0xffffffffu, cell[g], k);
                     const bool real = c >= 0 && ch * 8 < hd;
-                    cp16_or_zero(at + s * S::KV + swizzled(WA_KEYS, w * SHARE + g * 32 + k, ch), from + (real ? c + head + ch * 8 : 0), real);
+                    cp16_or_zero(stage + swizzled(WA_KEYS, w * SHARE + g * 32 + k, ch), from + (real ? c + head + ch * 8 : 0), real);
                 }
             over.issued(&full[s]);
         }
@@ -525,9 +594,11 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                             for (int k = 0; k < 32; k += 4) {
                                 float e[4];
 #pragma unroll
-                                for (int i4 = 0; i4 < 4; i4++) {
-                                    e[i4] = exp2_fast(fmaf(__uint_as_float(x[q][k + i4]), scale, -ref));
-                                    sum[i4] += e[i4];
+                                for (int i = 0; i < 4; i += 2) {
+                                    fma_pair(e[i], e[i + 1], __uint_as_float(x[q][k + i]), __uint_as_float(x[q][k + i + 1]), scale, -ref);
+                                    e[i] = exp2_fast(e[i]);
+                                    e[i + 1] = exp2_fast(e[i + 1]);
+                                    add_pair(sum[i], sum[i + 1], e[i], e[i + 1]);
                                 }
                                 p[k / 2] = pack2(e[0], e[1], T());
                                 p[k / 2 + 1] = pack2(e[2], e[3], T());
