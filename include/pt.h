@@ -101,6 +101,20 @@ void pt_disable_trace(pt_context_t *ctx);
 void pt_generate_greedy(pt_context_t *ctx, const int *prompt, int n_prompt,
                         int n_pos, int *out_tokens);
 
+/* A prompt in one pass: n tokens at ctx->pos on, which moves on by n. Returns
+ * the greedy token after the last one (state.logits are that position's, as
+ * after pt_forward_step), or -1 with ctx unchanged when the prompt does not
+ * fit seq_len, a token is outside the vocabulary, or the context is a shard
+ * (see ptc_decoder_prefill). */
+int pt_prefill(pt_context_t *ctx, const int *tokens, int n);
+
+/* pt_forward_step with the next token sampled on the GPU: temperature (0:
+ * greedy), top_k (0: off), top_p (1: off), min_p (0: off) from the caller's
+ * uniform random number u in [0, 1); the rules are ptc_sample_tokens'. The
+ * logits stay on the device unless ctx->sync_logits is set. */
+int pt_forward_step_sampled(pt_context_t *ctx, int token, float temperature,
+                            int top_k, float top_p, float min_p, float u);
+
 /* Copy device weights back into the caller's blob (after training). */
 void pt_sync_weights(pt_context_t *ctx);
 /* Fill ctx->grads._mem from the device gradients of the last step. */

@@ -152,6 +152,20 @@ int ptc_decoder_fetch_next(ptc_decoder *d, float *logits_host);
 void ptc_decoder_generate(ptc_decoder *d, const int *prompt, int n_prompt, int n_pos,
                           int *out_tokens);
 
+/* A prompt in one pass instead of one step per token: n tokens at positions
+ * pos0 on (positions before pos0 are in the cache), through batched products
+ * and the paged operators (ptc_serve.h) on the decoder's own cache. Returns
+ * the argmax after the last one, and its logits to logits_host if non-NULL,
+ * as a step of that token would; -1 (with a message) for a decoder without
+ * embedding, layers or head or with pipeline links, a head size that is no
+ * multiple of 8, tokens outside the vocabulary or more than the positions that
+ * are left. The first call takes buffers from the context's arena. */
+int ptc_decoder_prefill(ptc_decoder *d, const int *tokens, int n, int pos0, float *logits_host);
+/* One token sampled on the device from the last step's logits, by the rules
+ * of ptc_sample_tokens (ptc_serve.h; u uniform in [0, 1)). -1: no classifier,
+ * or no logit is a number. */
+int ptc_decoder_sample(ptc_decoder *d, float temperature, int top_k, float top_p, float min_p, float u);
+
 /* Benchmark hooks: enqueue the device-loop step graph n times without
  * synchronising (inputs already resident), and time it with CUDA events on
  * the decoder's stream. ptc_decoder_generate_begin loads the prompt and

@@ -164,6 +164,10 @@ def declare(L):
     _sig(L, "pt_free", None, ctx)
     _sig(L, "pt_forward_step", C.c_int, ctx, C.c_int)
     _sig(L, "pt_reset_kv", None, ctx)
+    _sig(L, "pt_prefill", C.c_int, ctx, i32p, C.c_int)
+    _sig(L, "pt_forward_step_sampled", C.c_int, ctx, C.c_int, C.c_float, C.c_int, C.c_float, C.c_float, C.c_float)
+    _sig(L, "ptc_decoder_prefill", C.c_int, vp, i32p, C.c_int, C.c_int, f32p)
+    _sig(L, "ptc_decoder_sample", C.c_int, vp, C.c_float, C.c_int, C.c_float, C.c_float, C.c_float)
     _sig(L, "pt_print_config", None, ctx)
     _sig(L, "pt_train_step", C.c_float, ctx, i32p, C.c_int, C.c_float)
     _sig(L, "pt_generate_greedy", None, ctx, i32p, C.c_int, C.c_int, i32p)
@@ -317,6 +321,17 @@ class Context:
 
     def forward_step(self, token):
         return self.L.pt_forward_step(C.byref(self.ctx), int(token))
+
+    def prefill(self, tokens):
+        """All of `tokens` in one pass (pt_prefill); the greedy token after the last."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int32)
+        nxt = self.L.pt_prefill(C.byref(self.ctx), ip(tokens), len(tokens))
+        if nxt < 0:
+            raise ValueError("pt_prefill refused the prompt")
+        return nxt
+
+    def forward_step_sampled(self, token, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        return self.L.pt_forward_step_sampled(C.byref(self.ctx), int(token), temperature, top_k, top_p, min_p, u)
 
     def logits(self):
         return np.ctypeslib.as_array(self.ctx.state.logits, shape=(self.cfg.vocab_size,)).copy()

@@ -254,6 +254,22 @@ int pt_forward_step(pt_context_t *ctx, int token) {
     return next;
 }
 
+int pt_prefill(pt_context_t *ctx, const int *tokens, int n) {
+    struct pt_device *d = ctx->dev;
+    if (!d) pt_fatal("pt_prefill on an uninitialised context");
+    pt_trace_begin(ctx->trace, "prefill", "fwd", -1);
+    int next = ptc_decoder_prefill(d->dec, tokens, n, ctx->pos, ctx->sync_logits ? ctx->state.logits : NULL);
+    pt_trace_end(ctx->trace);
+    if (next >= 0) ctx->pos += n;
+    return next;
+}
+
+int pt_forward_step_sampled(pt_context_t *ctx, int token, float temperature, int top_k, float top_p,
+                            float min_p, float u) {
+    int next = pt_forward_step(ctx, token);
+    return next < 0 ? next : ptc_decoder_sample(ctx->dev->dec, temperature, top_k, top_p, min_p, u);
+}
+
 /* pt.c:273-280. The cache that decodes read is the device one; the host
  * key_cache/value_cache buffers are never written by this library (they stay
  * as calloc left them), so clearing them -- 75 MB and ~10 ms for stories110M

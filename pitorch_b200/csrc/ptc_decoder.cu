@@ -9,14 +9,17 @@
 //   device graphs:  kernels only, for one position and for DEV_TOKENS
 //                   positions; position and token advance on the device, so
 //                   a whole greedy decode is a chain of graph launches.
+#include <math.h>
 #include <stddef.h>
 #include <stdio.h>
 #include <string.h>
 #include <time.h>
 
 #include "../../include/ptc.h"
+#include "../../include/ptc_serve.h"
 #include "ptc_common.cuh"
 #include "ptc_decode.cuh"
+#include "ptc_gemm.h"
 #include "ptc_internal.h"
 
 using ptc::DecodeModel;
@@ -29,7 +32,27 @@ struct HostIO {
     int err;   // the decode kernels' error word, fetched with next
 };
 
+// A prompt's pass (ptc_decoder_prefill): buffers of PREFILL_ROWS rows, made on
+// the first call.
+constexpr int PREFILL_ROWS = 256;
+struct Prefill {
+    float *x, *xm, *xn, *q, *k, *v, *qr, *att, *h1, *h3;
+    const float *rope;
+    int *in;        // tokens [PREFILL_ROWS], then past_len, new_len, free page
+    int *plan;      // page table, kv_len, q_start [2], pages used, err, then slots and positions
+    void *work;     // of the attention
+};
+
+// The rule and the result of one sampled step, pinned; the rule's device copy.
+struct SampleIO {
+    float temperature, top_p, min_p, u;
+    int top_k;
+    int token;
+};
+
 struct ptc_decoder {
+    Prefill *pre;
+    SampleIO *sample, *sample_dev;
     ptc_ctx *ctx;
     cudaStream_t stream;
     DecodeModel m;
@@ -174,6 +197,8 @@ extern "C" ptc_decoder *ptc_decoder_create(ptc_ctx *c, const ptc_config *cfg, co
                                            int has_embed, int has_head) {
     PTC_CHECK(cudaSetDevice(ptc_device(c)));
     ptc_decoder *d = new ptc_decoder();
+    d->pre = nullptr;
+    d->sample = d->sample_dev = nullptr;
     memset(&d->m, 0, sizeof(d->m));
     d->m.adv = 1;   // every single-token launch advances the device position
     d->m.link_recv = 1;   // a linked layer rank takes its input from its mailbox
@@ -338,6 +363,8 @@ extern "C" void ptc_decoder_destroy(ptc_decoder *d) {
     if (d->g_stage1) cudaGraphExecDestroy(d->g_stage1);
     ptc_host_free(d->io);
     ptc_host_free(d->stage);
+    ptc_host_free(d->sample);
+    delete d->pre;
     delete d;  // device buffers belong to the context arena
 }
 
@@ -661,4 +688,135 @@ extern "C" void ptc_decoder_enqueue_stage(ptc_decoder *d, int n) {
     int i = 0;
     for (; i + STAGE_POS <= n; i += STAGE_POS) PTC_CHECK(cudaGraphLaunch(d->g_stage, d->stream));
     for (; i < n; i++) PTC_CHECK(cudaGraphLaunch(d->g_stage1, d->stream));
+}
+
+// ---- a prompt in one pass, and sampled steps ----------------------------------
+
+static void make_prefill(ptc_decoder *d) {
+    if (d->pre) return;
+    const DecodeModel &m = d->m;
+    Prefill *p = new Prefill();
+    auto rows = [&](int width) { return (float *)ptc_alloc(d->ctx, (size_t)PREFILL_ROWS * width * 4); };
+    p->x = rows(m.dim);
+    p->xm = rows(m.dim);
+    p->xn = rows(m.dim);
+    p->q = rows(m.dim);
+    p->k = rows(m.kvd);
+    p->v = rows(m.kvd);
+    p->qr = rows(m.dim);
+    p->att = rows(m.dim);
+    p->h1 = rows(m.hidden);
+    p->h3 = rows(m.hidden);
+    p->rope = (const float *)m.rope;
+    if (!p->rope) {
+        float2 *t = (float2 *)ptc_alloc(d->ctx, (size_t)m.seq * (m.hd / 2) * sizeof(float2));
+        ptc::build_rope_table(t, m.seq, m.hd, d->stream);
+        p->rope = (const float *)t;
+    }
+    p->in = (int *)ptc_alloc(d->ctx, (PREFILL_ROWS + 3) * sizeof(int));
+    p->plan = (int *)ptc_alloc(d->ctx, (6 + 2 * PREFILL_ROWS) * sizeof(int));
+    p->work = ptc_alloc(d->ctx, PTC_ATTN_WORKSPACE_BYTES);
+    // the context's cache is one page of seq tokens per layer: page 0, free and in the table alike
+    PTC_CHECK(cudaMemsetAsync(p->in, 0, (PREFILL_ROWS + 3) * sizeof(int), d->stream));
+    PTC_CHECK(cudaMemsetAsync(p->plan, 0, (6 + 2 * PREFILL_ROWS) * sizeof(int), d->stream));
+    PTC_CHECK(cudaMemsetAsync(p->work, 0, PTC_ATTN_WORKSPACE_BYTES, d->stream));
+    d->pre = p;
+}
+
+static void prefill_gemm(const ptc_decoder *d, int rows, int N, int K, const float *A, const float *W, float *C, const float *R) {
+    ptc::GemmArgs g;
+    memset(&g, 0, sizeof(g));
+    g.M = rows; g.N = N; g.K = K;
+    g.A = A; g.lda = K; g.a_kcontig = true;
+    g.B = W; g.ldb = K; g.b_kcontig = true;
+    g.C = C; g.ldc = N;
+    g.R = R; g.ldr = N;
+    g.epi = R ? ptc::EPI_RESID : ptc::EPI_STORE;
+    ptc::gemm(g, d->n_sm, d->stream);
+}
+
+// Tokens [0, n) of d->pre->in through all layers, at the positions behind past_len. False: an operator refused.
+static bool prefill_rows(ptc_decoder *d, int n) {
+    const DecodeModel &m = d->m;
+    Prefill &p = *d->pre;
+    cudaStream_t s = d->stream;
+    int *table = p.plan, *kv_len = p.plan + 1, *q_start = p.plan + 2, *used = p.plan + 4, *err = p.plan + 5, *slots = p.plan + 6,
+        *positions = slots + PREFILL_ROWS, *past = p.in + PREFILL_ROWS;
+    const ptc_pages_args pages = {1, m.seq, 1, n, 1, 1, past, past + 1, past + 2, table, kv_len, q_start, slots, positions, used, err};
+    if (ptc_plan_pages(&pages, s)) return false;
+    ptc::launch_embed_rows(p.x, m.emb, p.in, n, m.dim, s);
+    for (int l = 0; l < m.L; l++) {
+        const size_t slab = (size_t)l * m.seq * m.kvd, dd = (size_t)m.dim * m.dim, kd = (size_t)m.kvd * m.dim, hd = (size_t)m.hidden * m.dim;
+        const ptc_paged_cache cache = {m.kc + slab, m.vc + slab, PTC_F32, 1, m.seq, m.nkv, m.hd, (long long)m.seq * m.kvd, (long long)m.seq * m.hd, m.hd};
+        ptc::launch_rmsnorm_rows(p.xn, p.x, m.rms_att + (size_t)l * m.dim, n, m.dim, s);
+        prefill_gemm(d, n, m.dim, m.dim, p.xn, m.wq + l * dd, p.q, nullptr);
+        prefill_gemm(d, n, m.kvd, m.dim, p.xn, m.wk + l * kd, p.k, nullptr);
+        prefill_gemm(d, n, m.kvd, m.dim, p.xn, m.wv + l * kd, p.v, nullptr);
+        const ptc_append_args app = {cache, n, m.nh, p.q, p.k, p.v, m.dim, m.kvd, m.kvd, positions, slots, p.rope, m.seq, p.qr, m.dim, err};
+        const ptc_attn_args att = {cache, 1, n, m.nh, n, 1, 0, 1.0f / sqrtf((float)m.hd), p.qr, m.dim, p.att, m.dim, table, kv_len, q_start,
+                                   p.work, PTC_ATTN_WORKSPACE_BYTES, err};
+        if (ptc_kv_append(&app, s) || ptc_paged_attention(&att, s)) return false;
+        prefill_gemm(d, n, m.dim, m.dim, p.att, m.wo + l * dd, p.xm, p.x);
+        ptc::launch_rmsnorm_rows(p.xn, p.xm, m.rms_ffn + (size_t)l * m.dim, n, m.dim, s);
+        prefill_gemm(d, n, m.hidden, m.dim, p.xn, m.w1 + l * hd, p.h1, nullptr);
+        prefill_gemm(d, n, m.hidden, m.dim, p.xn, m.w3 + l * hd, p.h3, nullptr);
+        ptc::launch_silu_rows(p.h1, p.h1, p.h3, (size_t)n * m.hidden, s);
+        prefill_gemm(d, n, m.dim, m.hidden, p.h1, m.w2 + l * hd, p.x, p.xm);
+    }
+    return true;
+}
+
+extern "C" int ptc_decoder_prefill(ptc_decoder *d, const int *tokens, int n, int pos0, float *logits_host) {
+    const DecodeModel &m = d->m;
+    const char *why = nullptr;
+    if (!d->has_embed || !d->has_head || m.L < 1) why = "a prompt needs the whole model";
+    else if (m.in_box) why = "not with pipeline links";
+    else if (m.hd % 8 || m.hd > 128) why = "head_dim has to be a multiple of 8, at most 128";
+    else if (!tokens || n < 1 || pos0 < 0 || n > m.seq - pos0) why = "the prompt does not fit the positions that are left";
+    else
+        for (int i = 0; i < n && !why; i++)
+            if (tokens[i] < 0 || tokens[i] >= m.V) why = "a token is outside the vocabulary";
+    if (why) {
+        fprintf(stderr, "pitorch_b200: ptc_decoder_prefill: %s\n", why);
+        return -1;
+    }
+    PTC_CHECK(cudaSetDevice(ptc_device(d->ctx)));
+    set_mode(d, 0);
+    make_prefill(d);
+    Prefill &p = *d->pre;
+    for (int done = 0; done < n; done += PREFILL_ROWS) {
+        const int rows = n - done < PREFILL_ROWS ? n - done : PREFILL_ROWS;
+        const int lens[2] = {pos0 + done, rows};
+        PTC_CHECK(cudaMemcpyAsync(p.in, tokens + done, rows * sizeof(int), cudaMemcpyHostToDevice, d->stream));
+        PTC_CHECK(cudaMemcpyAsync(p.in + PREFILL_ROWS, lens, sizeof(lens), cudaMemcpyHostToDevice, d->stream));
+        if (!prefill_rows(d, rows)) return -1;
+        if (done + rows == n)
+            PTC_CHECK(cudaMemcpyAsync(d->m.x, p.x + (size_t)(rows - 1) * m.dim, (size_t)m.dim * 4, cudaMemcpyDeviceToDevice, d->stream));
+    }
+    int err = 0;
+    PTC_CHECK(cudaMemcpyAsync(&err, p.plan + 5, sizeof(int), cudaMemcpyDeviceToHost, d->stream));
+    ptc_decoder_enqueue_head(d);
+    const int next = ptc_decoder_fetch_next(d, logits_host);
+    if (err) PTC_FATAL("prompt kernels reported error %d", err);
+    return next;
+}
+
+extern "C" int ptc_decoder_sample(ptc_decoder *d, float temperature, int top_k, float top_p, float min_p, float u) {
+    if (!d->has_head) {
+        fprintf(stderr, "pitorch_b200: ptc_decoder_sample: no classifier\n");
+        return -1;
+    }
+    PTC_CHECK(cudaSetDevice(ptc_device(d->ctx)));
+    if (!d->sample) {
+        d->sample = (SampleIO *)ptc_host_alloc(sizeof(SampleIO));
+        d->sample_dev = (SampleIO *)ptc_alloc(d->ctx, sizeof(SampleIO));
+    }
+    *d->sample = {temperature, top_p, min_p, u, top_k, -1};
+    SampleIO *s = d->sample_dev;
+    PTC_CHECK(cudaMemcpyAsync(s, d->sample, sizeof(SampleIO), cudaMemcpyHostToDevice, d->stream));
+    const ptc_sample_args a = {PTC_F32, 1, d->m.V, d->m.logits, d->m.V, &s->temperature, &s->top_k, &s->top_p, &s->min_p, &s->u, &s->token};
+    if (ptc_sample_tokens(&a, d->stream)) return -1;
+    PTC_CHECK(cudaMemcpyAsync(&d->sample->token, &s->token, sizeof(int), cudaMemcpyDeviceToHost, d->stream));
+    PTC_CHECK(cudaStreamSynchronize(d->stream));
+    return d->sample->token;
 }

@@ -32,6 +32,10 @@ int decode_attn_stage(int dim, int nh, int nkv, int seq);
 // The decoder's RoPE table; the launch form reports a failure, the other aborts on it.
 cudaError_t launch_rope_table(float2 *t, int seq, int hd, cudaStream_t s);
 void build_rope_table(float2 *t, int seq, int hd, cudaStream_t s);
+// Rows of a prompt (ptc_train.cu): embedding lookups, rmsnorm, silu(h1) * h3.
+void launch_embed_rows(float *out, const float *emb, const int *tokens, int rows, int D, cudaStream_t s);
+void launch_rmsnorm_rows(float *out, const float *x, const float *w, int rows, int D, cudaStream_t s);
+void launch_silu_rows(float *out, const float *h1, const float *h3, size_t n, cudaStream_t s);
 void transpose_w2(const DecodeModel &m, float *w2t, cudaStream_t s);
 // host_next: pinned host word that also receives the argmax (or null).
 void launch_head(const DecodeModel &m, int n_sm, cudaStream_t s, int *host_next = nullptr);

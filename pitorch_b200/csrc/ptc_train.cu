@@ -568,6 +568,20 @@ __global__ void k_tr_sgd(float *w, const float *g, size_t n, float lr) {
         w[e] = __fsub_rn(w[e], __fmul_rn(lr, g[e]));
 }
 
+// The row kernels for the prompt's pass of a decoder (ptc_decoder_prefill).
+void launch_embed_rows(float *out, const float *emb, const int *tokens, int rows, int D, cudaStream_t s) {
+    k_tr_embed<<<(rows * D + 255) / 256, 256, 0, s>>>(out, emb, tokens, rows, D);
+    PTC_CHECK(cudaGetLastError());
+}
+void launch_rmsnorm_rows(float *out, const float *x, const float *w, int rows, int D, cudaStream_t s) {
+    k_tr_rmsnorm<<<(rows + 7) / 8, 256, 0, s>>>(out, x, w, rows, D);
+    PTC_CHECK(cudaGetLastError());
+}
+void launch_silu_rows(float *out, const float *h1, const float *h3, size_t n, cudaStream_t s) {
+    k_tr_silu_gate<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(out, h1, h3, n);
+    PTC_CHECK(cudaGetLastError());
+}
+
 }  // namespace ptc
 
 // ---------------------------------------------------------------------------
