@@ -23,6 +23,7 @@ constexpr int NA_THREADS = NA_WARPS * 32;
 constexpr int NA_KEYS = 16;                   // keys of a warp's stage
 constexpr int NA_UNIT = NA_WARPS * NA_KEYS;   // keys of a unit
 constexpr int NA_STAGES = 3;
+constexpr int NA_MAX_CTAS = 444;               // three per SM: the parts that one item can have
 
 template <typename T, int HDP, int MT>
 struct NarrowShape {
@@ -291,24 +292,6 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
     for (int u = attn_first(c, C, total); u < u1;) {
         const AttnItem it = attn_find<MT, NA_UNIT>(a, group, pre, u);
         const int seg0 = u - it.first, seg1 = min(it.units, seg0 + u1 - u), rows = it.i1 - it.i0;
-        if constexpr (sizeof(T) == 4) {
-            int *lim = (int *)(qs + MT * HDP);
-            for (int i = tid; i < MT * HDP; i += NA_THREADS) {
-                const int r = i / HDP, d = i % HDP, row = it.i0 + r, tok = row / group;
-                qs[i] = r < rows && d < hd ? Elem<T>::up(((const T *)a.q)[(it.s.q0 + tok) * a.q_stride +
-                                                                         (long long)(it.head * group + row - tok * group) * hd + d])
-                                           : 0.f;
-            }
-            if (tid < MT) {
-                const int pos = it.s.pos0 + (it.i0 + tid) / group;
-                lim[tid] = a.window > 0 ? pos - a.window + 1 : 0;
-                lim[MT + tid] = tid < rows ? min(pos + 1, it.s.cap) : 0;
-            }
-            __syncthreads();
-        }
-        NarrowRows<T, HDP, MT> st;
-        st.begin(a, it, group, qs);
-
         // This warp's keys: 16 of every unit. Lanes 0..15 look up a key each.
         const int n = seg1 - seg0, key0 = (it.lo / NA_UNIT + seg0) * NA_UNIT + warp * NA_KEYS;
         const int *table = a.page_table + (long long)it.r * a.max_pages;
@@ -348,6 +331,24 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
 #pragma unroll
         for (int j = 0; j < NA_STAGES - 1; j++) there[j] = fill(j, pages[j]);
         int page = pages[NA_STAGES - 1];
+        // the queries, while the first keys are on their way
+        if constexpr (sizeof(T) == 4) {
+            int *lim = (int *)(qs + MT * HDP);
+            for (int i = tid; i < MT * HDP; i += NA_THREADS) {
+                const int r = i / HDP, d = i % HDP, row = it.i0 + r, tok = row / group;
+                qs[i] = r < rows && d < hd ? Elem<T>::up(((const T *)a.q)[(it.s.q0 + tok) * a.q_stride +
+                                                                         (long long)(it.head * group + row - tok * group) * hd + d])
+                                           : 0.f;
+            }
+            if (tid < MT) {
+                const int pos = it.s.pos0 + (it.i0 + tid) / group;
+                lim[tid] = a.window > 0 ? pos - a.window + 1 : 0;
+                lim[MT + tid] = tid < rows ? min(pos + 1, it.s.cap) : 0;
+            }
+            __syncthreads();
+        }
+        NarrowRows<T, HDP, MT> st;
+        st.begin(a, it, group, qs);
         for (int j = 0; j < n; j++) {
             cp_async_wait<NA_STAGES - 2>();
             __syncwarp();
@@ -409,31 +410,59 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
             }
             __syncthreads();
             if (last) {
-                for (int i = tid; i < rows * (HDP / 4); i += NA_THREADS) {
-                    const int r = i / (HDP / 4), d = i % (HDP / 4) * 4;
-                    if (d >= hd) continue;
+                // weights of the parts, a warp per row and a lane per part; then the
+                // weighted sum, the parts shared out where there are few rows
+                const int parts = c1 - c0 + 1;
+                float *wgt = ow, *red = ow + (MT * parts + 3) / 4 * 4;
+                auto part = [&](int p) { return slots + (long long)(2 * (c0 + p) + (p == 0)) * SLOT; };
+                for (int r = warp; r < rows; r += NA_WARPS) {
                     float top = -INFINITY, sum = 0.f;
-                    for (int p = c0; p <= c1; p++) top = fmaxf(top, __ldcg(slots + (long long)(2 * p + (p == c0)) * SLOT + MT * HDP + r));
+                    for (int p = lane; p < parts; p += 32) top = fmaxf(top, __ldcg(part(p) + MT * HDP + r));
+                    top = warp_max(top);
                     const float ref = top == -INFINITY ? 0.f : top;
+                    for (int p = lane; p < parts; p += 32) {
+                        const float f = exp2f(__ldcg(part(p) + MT * HDP + r) - ref);
+                        wgt[r * parts + p] = f;
+                        sum += f * __ldcg(part(p) + MT * HDP + MT + r);
+                    }
+                    sum = warp_sum(sum);
+                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                    for (int p = lane; p < parts; p += 32) wgt[r * parts + p] *= inv;
+                }
+                __syncthreads();
+                const int cols = rows * (HDP / 4), shares = max(1, NA_THREADS / cols);
+                for (int i = tid; i < cols * shares; i += NA_THREADS) {
+                    const int share = i / cols, x = i % cols, r = x / (HDP / 4), d = x % (HDP / 4) * 4;
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-                    for (int p = c0; p <= c1; p++) {
-                        const float *from = slots + (long long)(2 * p + (p == c0)) * SLOT;
-                        const float f = exp2f(__ldcg(from + MT * HDP + r) - ref);
-                        const float4 x = __ldcg((const float4 *)(from + r * HDP + d));
-                        sum += f * __ldcg(from + MT * HDP + MT + r);
-                        acc.x += f * x.x;
-                        acc.y += f * x.y;
-                        acc.z += f * x.z;
-                        acc.w += f * x.w;
+                    for (int p = share; p < parts; p += shares) {
+                        const float f = wgt[r * parts + p];
+                        const float4 v = __ldcg((const float4 *)(part(p) + r * HDP + d));
+                        acc.x += f * v.x;
+                        acc.y += f * v.y;
+                        acc.z += f * v.z;
+                        acc.w += f * v.w;
                     }
-                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+                    *(float4 *)(red + i * 4) = acc;
+                }
+                __syncthreads();
+                for (int x = tid; x < cols; x += NA_THREADS) {
+                    const int r = x / (HDP / 4), d = x % (HDP / 4) * 4;
+                    if (d >= hd) continue;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int share = 0; share < shares; share++) {
+                        const float4 v = *(const float4 *)(red + (share * cols + x) * 4);
+                        acc.x += v.x;
+                        acc.y += v.y;
+                        acc.z += v.z;
+                        acc.w += v.w;
+                    }
                     const int row = it.i0 + r, tok = row / group;
                     T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + row - tok * group) * hd + d;
-                    dst[0] = Elem<T>::down(acc.x * inv);
-                    dst[1] = Elem<T>::down(acc.y * inv);
-                    dst[2] = Elem<T>::down(acc.z * inv);
-                    dst[3] = Elem<T>::down(acc.w * inv);
+                    dst[0] = Elem<T>::down(acc.x);
+                    dst[1] = Elem<T>::down(acc.y);
+                    dst[2] = Elem<T>::down(acc.z);
+                    dst[3] = Elem<T>::down(acc.w);
                 }
                 if (tid == 0) flags[c0] = 0;
             }
@@ -448,6 +477,9 @@ static cudaError_t launch_narrow(const ptc_attn_args &a, int group, int n_sm, cu
     auto kernel = k_attn_narrow<T, HDP, MT>;
     const int smem = NA_WARPS * NarrowShape<T, HDP, MT>::WARP + (a.n_seqs + 1) * (int)sizeof(int);
     static_assert(NA_WARPS * MT * HDP * 4 <= NA_WARPS * NarrowShape<T, HDP, MT>::WARP, "the outputs fit the stages");
+    // (and so do a merge's weights and sums: MT a part, of at most the CTAs, and 4 floats a thread or an output)
+    static_assert((MT * NA_MAX_CTAS + 3) * 4 + 4 * (NA_THREADS > MT * HDP / 4 ? NA_THREADS : MT * HDP / 4) * 4 <=
+                      NA_WARPS * NarrowShape<T, HDP, MT>::WARP, "a merge fits the stages");
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     int per = 0;
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, NA_THREADS, smem);
@@ -456,7 +488,8 @@ static cudaError_t launch_narrow(const ptc_attn_args &a, int group, int n_sm, cu
     int grid = per * n_sm;
     const long long fit = (long long)(PTC_ATTN_WORKSPACE_BYTES - ATTN_FLAG_BYTES) / (2 * NarrowShape<T, HDP, MT>::SLOT * sizeof(float));
     if (grid > fit) grid = (int)fit;
-    if (grid > ATTN_FLAG_BYTES / 4) grid = ATTN_FLAG_BYTES / 4;
+    if (grid > NA_MAX_CTAS) grid = NA_MAX_CTAS;
+    static_assert(NA_MAX_CTAS <= ATTN_FLAG_BYTES / 4, "a counter per CTA");
     kernel<<<grid, NA_THREADS, smem, s>>>(a, group);
     return cudaGetLastError();
 }
