@@ -35,13 +35,6 @@ struct NarrowShape {
     static constexpr int SLOT = (MT * (HDP + 2) + 3) / 4 * 4;
 };
 
-__device__ __forceinline__ void cp_async16_or_zero(unsigned dst, const void *src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], unsigned at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -404,66 +397,11 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
             const int c0 = attn_owner(it.first, C, total), c1 = attn_owner(it.first + it.units - 1, C, total);
             __syncthreads();
             if (tid == 0) {
-                __threadfence();
                 last = atom_add_acq_rel(&flags[c0], 1u) == (unsigned)(c1 - c0);
-                __threadfence();
             }
             __syncthreads();
             if (last) {
-                // weights of the parts, a warp per row and a lane per part; then the
-                // weighted sum, the parts shared out where there are few rows
-                const int parts = c1 - c0 + 1;
-                float *wgt = ow, *red = ow + (MT * parts + 3) / 4 * 4;
-                auto part = [&](int p) { return slots + (long long)(2 * (c0 + p) + (p == 0)) * SLOT; };
-                for (int r = warp; r < rows; r += NA_WARPS) {
-                    float top = -INFINITY, sum = 0.f;
-                    for (int p = lane; p < parts; p += 32) top = fmaxf(top, __ldcg(part(p) + MT * HDP + r));
-                    top = warp_max(top);
-                    const float ref = top == -INFINITY ? 0.f : top;
-                    for (int p = lane; p < parts; p += 32) {
-                        const float f = exp2f(__ldcg(part(p) + MT * HDP + r) - ref);
-                        wgt[r * parts + p] = f;
-                        sum += f * __ldcg(part(p) + MT * HDP + MT + r);
-                    }
-                    sum = warp_sum(sum);
-                    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-                    for (int p = lane; p < parts; p += 32) wgt[r * parts + p] *= inv;
-                }
-                __syncthreads();
-                const int cols = rows * (HDP / 4), shares = max(1, NA_THREADS / cols);
-                for (int i = tid; i < cols * shares; i += NA_THREADS) {
-                    const int share = i / cols, x = i % cols, r = x / (HDP / 4), d = x % (HDP / 4) * 4;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int p = share; p < parts; p += shares) {
-                        const float f = wgt[r * parts + p];
-                        const float4 v = __ldcg((const float4 *)(part(p) + r * HDP + d));
-                        acc.x += f * v.x;
-                        acc.y += f * v.y;
-                        acc.z += f * v.z;
-                        acc.w += f * v.w;
-                    }
-                    *(float4 *)(red + i * 4) = acc;
-                }
-                __syncthreads();
-                for (int x = tid; x < cols; x += NA_THREADS) {
-                    const int r = x / (HDP / 4), d = x % (HDP / 4) * 4;
-                    if (d >= hd) continue;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int share = 0; share < shares; share++) {
-                        const float4 v = *(const float4 *)(red + (share * cols + x) * 4);
-                        acc.x += v.x;
-                        acc.y += v.y;
-                        acc.z += v.z;
-                        acc.w += v.w;
-                    }
-                    const int row = it.i0 + r, tok = row / group;
-                    T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + row - tok * group) * hd + d;
-                    dst[0] = Elem<T>::down(acc.x);
-                    dst[1] = Elem<T>::down(acc.y);
-                    dst[2] = Elem<T>::down(acc.z);
-                    dst[3] = Elem<T>::down(acc.w);
-                }
+                attn_merge<T, HDP, MT, SLOT, NA_THREADS>(a, it, group, slots, c0, c1, ow);
                 if (tid == 0) flags[c0] = 0;
             }
         }
@@ -533,7 +471,8 @@ extern "C" int ptc_paged_attention(const ptc_attn_args *p, void *stream) {
     const long long most = (long long)(a.max_q < 1 ? 1 : a.max_q) * group;   // rows of a K/V head
     if (a.cache.dtype == PTC_F32) {
         // rows in registers: as many as the longest sequence fills, up to 8
-        if (most <= 1) SERVE_CUDA((ptc::launch_narrow_hd<float, 1>(a, group, n_sm, s)));
+        if (most > 16) SERVE_CUDA(ptc::launch_attn_f32(a, group, n_sm, s));
+        else if (most <= 1) SERVE_CUDA((ptc::launch_narrow_hd<float, 1>(a, group, n_sm, s)));
         else if (most <= 4) SERVE_CUDA((ptc::launch_narrow_hd<float, 4>(a, group, n_sm, s)));
         else SERVE_CUDA((ptc::launch_narrow_hd<float, 8>(a, group, n_sm, s)));
     } else if (most > 64 && a.scale > 0.f) {

@@ -211,9 +211,6 @@ struct Handover {
     }
 };
 
-__device__ __forceinline__ void cp16_or_zero(unsigned dst, const void *src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
 // Where 16-byte chunk `ch` of row `row` lies in a tile of `rows` rows.
 __device__ __forceinline__ unsigned swizzled(int rows, int row, int ch) {
     return (unsigned)((ch >> 3) * rows * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
@@ -257,7 +254,7 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
                 const int row = x / CH, ch = x % CH, i = it.i0 + row, tok = i / group;
                 const bool real = i < it.i1 && ch * 8 < hd;
                 const long long off = real ? (it.s.q0 + tok) * a.q_stride + (long long)(it.head * group + i - tok * group) * hd + ch * 8 : 0;
-                cp16_or_zero(q_at + (row >> 7) * (S::Q / 2) + swizzled(WA_TILE, row & 127, ch), (const T *)a.q + off, real);
+                cp_async16_or_zero(q_at + (row >> 7) * (S::Q / 2) + swizzled(WA_TILE, row & 127, ch), (const T *)a.q + off, real);
             }
             over.issued(&sh.bar.q_full);
         }
@@ -334,7 +331,7 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
                     for (int x = lane; x < run * CH; x += 32) {
                         const int k = x / CH, ch = x % CH;
                         const bool real = te + k < it.hi && ch * 8 < hd;
-                        cp16_or_zero(stage + swizzled(WA_KEYS, k0 + k, ch), from + (real ? cell + k * a.cache.token_stride + head + ch * 8 : 0), real);
+                        cp_async16_or_zero(stage + swizzled(WA_KEYS, k0 + k, ch), from + (real ? cell + k * a.cache.token_stride + head + ch * 8 : 0), real);
                     }
                     over.issued(&full[s]);
                 } else {
@@ -370,7 +367,7 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
                     const int x = i * 32 + lane, k = x / CH, ch = x % CH;
                     const long long c = __shfl_sync(0xffffffffu, cell[g], k);
                     const bool real = c >= 0 && ch * 8 < hd;
-                    cp16_or_zero(stage + swizzled(WA_KEYS, w * SHARE + g * 32 + k, ch), from + (real ? c + head + ch * 8 : 0), real);
+                    cp_async16_or_zero(stage + swizzled(WA_KEYS, w * SHARE + g * 32 + k, ch), from + (real ? c + head + ch * 8 : 0), real);
                 }
             over.issued(&full[s]);
         }
@@ -656,9 +653,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                 const int c0 = attn_owner(it.first, C, total), c1 = attn_owner(it.first + it.units - 1, C, total);
                 bar_sync(1, WA_ROWS);
                 if (tid == 0) {
-                    __threadfence();
                     sh.last = atom_add_acq_rel(&flags[c0], 1u) == (unsigned)(c1 - c0);
-                    __threadfence();
                 }
                 bar_sync(1, WA_ROWS);
                 if (sh.last) {
