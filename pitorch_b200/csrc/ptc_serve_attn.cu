@@ -23,6 +23,10 @@ constexpr int NA_THREADS = NA_WARPS * 32;
 constexpr int NA_KEYS = 16;                   // keys of a warp's stage
 constexpr int NA_UNIT = NA_WARPS * NA_KEYS;   // keys of a unit
 constexpr int NA_STAGES = 3;
+// A row's reference for its probabilities is raised only when a score passes it
+// by this (sums and outputs are relative to the same value, and stay below 2^8
+// times the keys' number).
+constexpr float NA_RISE = 8.f;
 constexpr int NA_MAX_CTAS = 444;               // three per SM: the parts that one item can have
 
 template <typename T, int HDP, int MT>
@@ -106,10 +110,9 @@ struct NarrowRows {
             mma16816(s[0], q[k], b[0], b[1], T());
             mma16816(s[1], q[k], b[2], b[3], T());
         }
-        float f[2];
+        float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float top = m[h];
+        for (int h = 0; h < 2; h++)
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -118,23 +121,32 @@ struct NarrowRows {
                     const bool see = t < hi[h] && t >= lo[h] && (there >> c & 1);
                     float &v = s[n][2 * h + e];
                     v = see ? v * scale : -INFINITY;
-                    top = fmaxf(top, v);
+                    top[h] = fmaxf(top[h], v);
                 }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const float ref = top == -INFINITY ? 0.f : top;
-            f[h] = exp2f(m[h] - ref);
-            m[h] = top;
-            float add = 0.f;
+        if (__any_sync(0xffffffffu, top[0] > m[0] + NA_RISE || top[1] > m[1] + NA_RISE)) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float t = fmaxf(top[h], m[h]);
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                const float f = t == -INFINITY ? 0.f : exp2f(m[h] - t);
+                m[h] = t;
+                l[h] *= f;
+#pragma unroll
+                for (int n = 0; n < HDP / 8; n++) o[n][2 * h] *= f, o[n][2 * h + 1] *= f;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const float ref = m[h] == -INFINITY ? 0.f : m[h];
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     float &v = s[n][2 * h + e];
-                    v = exp2f(v - ref);
-                    add += v;
+                    v = exp2_fast(v - ref);
+                    l[h] += v;
                 }
-            l[h] = l[h] * f[h] + add;
         }
         // probabilities rounded to the type for the product with V, as one operand type has to be (their sum is not)
         const uint32_t p[4] = {pack2(s[0][0], s[0][1], T()), pack2(s[0][2], s[0][3], T()), pack2(s[1][0], s[1][1], T()),
@@ -147,10 +159,6 @@ struct NarrowRows {
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 float(&c)[4] = o[2 * n + x];
-                c[0] *= f[0];
-                c[1] *= f[0];
-                c[2] *= f[1];
-                c[3] *= f[1];
                 mma16816(c, p, b[2 * x], b[2 * x + 1], T());
             }
         }
@@ -206,28 +214,34 @@ struct NarrowRows<float, HDP, MT> {
 #pragma unroll
             for (int r = 0; r < MT; r++) s[r] = dot4(x, *(const float4 *)(qs + r * HDP + (c + half) * 4), s[r]);
         }
-        float f[MT];
         const int t = key + k;
+        bool rise = false;
 #pragma unroll
         for (int r = 0; r < MT; r++) {
-            float v = s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16);
-            v = t < hi[r] && t >= lo[r] && (there >> k & 1) ? v * scale : -INFINITY;
-            float top = v;
+            s[r] += __shfl_xor_sync(0xffffffffu, s[r], 16);
+            s[r] = t < hi[r] && t >= lo[r] && (there >> k & 1) ? s[r] * scale : -INFINITY;
+            rise |= s[r] > m[r] + NA_RISE;
+        }
+        if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
-            for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            top = fmaxf(top, m[r]);
-            const float ref = top == -INFINITY ? 0.f : top;
-            f[r] = exp2f(m[r] - ref);
-            m[r] = top;
-            const float p = exp2f(v - ref);
-            l[r] = l[r] * f[r] + p;   // of this lane's keys
+            for (int r = 0; r < MT; r++) {
+                float top = fmaxf(s[r], m[r]);
+#pragma unroll
+                for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float f = top == -INFINITY ? 0.f : exp2f(m[r] - top);
+                m[r] = top;
+                l[r] *= f;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[r][e] *= f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < MT; r++) {
+            const float p = exp2_fast(s[r] - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] += p;   // of this lane's keys
             if (half == 0) ps[r * NA_KEYS + k] = p;
         }
         __syncwarp();
-#pragma unroll
-        for (int r = 0; r < MT; r++)
-#pragma unroll
-            for (int e = 0; e < E; e++) o[r][e] *= f[r];
 #pragma unroll
         for (int j = 0; j < NA_KEYS; j += 4) {
             float v[4][E];

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, int gr
                 l[i] *= f;
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    const float p = exp2f(s[i][b] - ref);
+                    const float p = exp2_fast(s[i][b] - ref);
                     l[i] += p;
                     ps[(ty * 4 + i) * S::P_ROW + tx + 16 * b] = p;
                 }
