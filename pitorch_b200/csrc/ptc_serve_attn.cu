@@ -70,14 +70,14 @@ struct NarrowRows {
     float m[2], l[2];
     int lo[2], hi[2];
 
-    __device__ void begin(const ptc_attn_args &a, const AttnItem &it, int group, const float *) {
+    __device__ void begin(const ptc_attn_args &a, const AttnItem &it, Group group, const float *) {
         const int lane = threadIdx.x & 31, hd = a.cache.head_dim;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int i = it.i0 + lane / 4 + 8 * h, tok = i / group;
+            const int i = it.i0 + lane / 4 + 8 * h, tok = group.div(i);
             const bool real = i < it.i1;
             const T *src = (const T *)a.q + (it.s.q0 + (real ? tok : 0)) * a.q_stride +
-                           (long long)(it.head * group + (real ? i - tok * group : 0)) * hd;
+                           (long long)(it.head * group.n + (real ? i - tok * group.n : 0)) * hd;
 #pragma unroll
             for (int k = 0; k < HDP / 16; k++)
 #pragma unroll
@@ -189,7 +189,7 @@ struct NarrowRows<float, HDP, MT> {
     static constexpr int E = HDP / 32;
     float o[MT][E], m[MT], l[MT];
 
-    __device__ void begin(const ptc_attn_args &, const AttnItem &, int, const float *) {
+    __device__ void begin(const ptc_attn_args &, const AttnItem &, Group, const float *) {
 #pragma unroll
         for (int r = 0; r < MT; r++) {
             m[r] = -INFINITY;
@@ -275,7 +275,7 @@ struct NarrowRows<float, HDP, MT> {
 };
 
 template <typename T, int HDP, int MT>
-__global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int group) {
+__global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, Group group) {
     using S = NarrowShape<T, HDP, MT>;
     constexpr int SLOT = S::SLOT;
     extern __shared__ __align__(16) char na_smem[];
@@ -342,13 +342,13 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
         if constexpr (sizeof(T) == 4) {
             int *lim = (int *)(qs + MT * HDP);
             for (int i = tid; i < MT * HDP; i += NA_THREADS) {
-                const int r = i / HDP, d = i % HDP, row = it.i0 + r, tok = row / group;
+                const int r = i / HDP, d = i % HDP, row = it.i0 + r, tok = group.div(row);
                 qs[i] = r < rows && d < hd ? Elem<T>::up(((const T *)a.q)[(it.s.q0 + tok) * a.q_stride +
-                                                                         (long long)(it.head * group + row - tok * group) * hd + d])
+                                                                         (long long)(it.head * group.n + row - tok * group.n) * hd + d])
                                            : 0.f;
             }
             if (tid < MT) {
-                const int pos = it.s.pos0 + (it.i0 + tid) / group;
+                const int pos = it.s.pos0 + group.div(it.i0 + tid);
                 lim[tid] = a.window > 0 ? pos - a.window + 1 : 0;
                 lim[MT + tid] = tid < rows ? min(pos + 1, it.s.cap) : 0;
             }
@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
             }
             if (whole) {
                 const float inv = sum > 0.f ? 1.f / sum : 0.f;
-                const int row = it.i0 + r, tok = row / group;
-                T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + row - tok * group) * hd + d;
+                const int row = it.i0 + r, tok = group.div(row);
+                T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group.n + row - tok * group.n) * hd + d;
                 dst[0] = Elem<T>::down(acc.x * inv);
                 dst[1] = Elem<T>::down(acc.y * inv);
                 dst[2] = Elem<T>::down(acc.z * inv);
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, int
 }
 
 template <typename T, int HDP, int MT>
-static cudaError_t launch_narrow(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+static cudaError_t launch_narrow(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     auto kernel = k_attn_narrow<T, HDP, MT>;
     const int smem = NA_WARPS * NarrowShape<T, HDP, MT>::WARP + (a.n_seqs + 1) * (int)sizeof(int);
     static_assert(NA_WARPS * MT * HDP * 4 <= NA_WARPS * NarrowShape<T, HDP, MT>::WARP, "the outputs fit the stages");
@@ -447,7 +447,7 @@ static cudaError_t launch_narrow(const ptc_attn_args &a, int group, int n_sm, cu
 }
 
 template <typename T, int MT>
-static cudaError_t launch_narrow_hd(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+static cudaError_t launch_narrow_hd(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     const int hd = a.cache.head_dim;
     if (hd <= 32) return launch_narrow<T, 32, MT>(a, group, n_sm, s);
     if (hd <= 64) return launch_narrow<T, 64, MT>(a, group, n_sm, s);
@@ -481,8 +481,8 @@ extern "C" int ptc_paged_attention(const ptc_attn_args *p, void *stream) {
     SERVE_CUDA(on.error());
     int n_sm = 0;
     SERVE_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, on.device()));
-    const int group = a.n_heads / a.cache.n_kv_heads;
-    const long long most = (long long)(a.max_q < 1 ? 1 : a.max_q) * group;   // rows of a K/V head
+    const ptc::Group group(a.n_heads / a.cache.n_kv_heads);
+    const long long most = (long long)(a.max_q < 1 ? 1 : a.max_q) * group.n;   // rows of a K/V head
     if (a.cache.dtype == PTC_F32) {
         // rows in registers: as many as the longest sequence fills, up to 8
         if (most > 16) SERVE_CUDA(ptc::launch_attn_f32(a, group, n_sm, s));

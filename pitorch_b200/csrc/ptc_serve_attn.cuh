@@ -2,7 +2,7 @@
 // kernels).
 //
 // An item is (sequence, K/V head, row tile): the query heads of one K/V head
-// are packed as rows, row i = token i / group, head i % group, and a tile has
+// are packed as rows, row i = token group.div(i), head i % group, and a tile has
 // a fixed number of them, so a key that is read serves them all. An item's
 // work is counted in units of a fixed number of keys, and the units of all
 // items, laid end to end, are cut into one equal range per CTA. So one long
@@ -24,6 +24,19 @@ namespace ptc {
 constexpr int ATTN_MAX_SEQS = PTC_SERVE_MAX_SEQS;
 constexpr int ATTN_FLAG_BYTES = 4096;   // counters at the front of the workspace, one per CTA
 constexpr float LOG2E = 1.4426950408889634f;
+
+// Query heads of a K/V head, and division by their number: by a multiplication
+// with floor(2^32 / n) + 1, which is at most one too high below 2^31.
+struct Group {
+    int n;
+    unsigned magic;
+    explicit Group(int heads) : n(heads), magic(heads > 1 ? (unsigned)((1ull << 32) / heads) + 1 : 0) {}
+    __device__ __forceinline__ int div(int i) const {
+        if (n == 1) return i;
+        const int q = (int)__umulhi((unsigned)i, magic);
+        return q * n > i ? q - 1 : q;
+    }
+};
 
 // One sequence as the kernels use it; bad lengths give no rows.
 struct AttnSeq {
@@ -48,17 +61,17 @@ __device__ __forceinline__ AttnSeq attn_seq(const ptc_attn_args &a, int r) {
     return s;
 }
 
-// The keys [lo, hi) that rows [i0, i1) of a sequence see (i = token * group + head).
-__device__ __forceinline__ void attn_keys(const AttnSeq &s, int group, int window, int i0, int i1, int &lo, int &hi) {
-    hi = min(s.pos0 + (i1 - 1) / group + 1, s.cap);
-    lo = window > 0 ? max(0, s.pos0 + i0 / group - window + 1) : 0;
+// The keys [lo, hi) that rows [i0, i1) of a sequence see (i = token * group.n + head).
+__device__ __forceinline__ void attn_keys(const AttnSeq &s, Group group, int window, int i0, int i1, int &lo, int &hi) {
+    hi = min(s.pos0 + group.div(i1 - 1) + 1, s.cap);
+    lo = window > 0 ? max(0, s.pos0 + group.div(i0) - window + 1) : 0;
 }
 
 // Units of row tile m of a sequence: one at least, so that rows that see nothing are written.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ int attn_units(const AttnSeq &s, int group, int window, int m) {
+__device__ __forceinline__ int attn_units(const AttnSeq &s, Group group, int window, int m) {
     int lo, hi;
-    attn_keys(s, group, window, m * ROWS, min(s.n * group, (m + 1) * ROWS), lo, hi);
+    attn_keys(s, group, window, m * ROWS, min(s.n * group.n, (m + 1) * ROWS), lo, hi);
     return hi > lo ? (hi + KEYS - 1) / KEYS - lo / KEYS : 1;
 }
 
@@ -66,7 +79,7 @@ __device__ __forceinline__ int attn_units(const AttnSeq &s, int group, int windo
 // threads of the CTA; pre[n_seqs] is the total. scratch: THREADS / 32 ints. A
 // total past 2^31 / heads leaves nothing to do (LENGTH).
 template <int ROWS, int KEYS, int THREADS>
-__device__ void attn_prefix(const ptc_attn_args &a, int group, int *pre, long long *scratch) {
+__device__ void attn_prefix(const ptc_attn_args &a, Group group, int *pre, long long *scratch) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n_seqs;
     const int per = (n + THREADS - 1) / THREADS, r0 = min(n, tid * per);
     long long sum = 0;
@@ -77,7 +90,7 @@ __device__ void attn_prefix(const ptc_attn_args &a, int group, int *pre, long lo
         AttnSeq s = {0, 0, 0, 0, 0};
         if (mine) s = attn_seq(a, r);
         bad |= s.bad;
-        const long long rows = (long long)s.n * group;
+        const long long rows = (long long)s.n * group.n;
         const int tiles = (int)((rows + ROWS - 1) / ROWS);
         long long u = 0;
         if (tiles <= 8)
@@ -144,7 +157,7 @@ struct AttnItem {
 
 // The item that holds unit u. All threads of a CTA get the same.
 template <int ROWS, int KEYS>
-__device__ AttnItem attn_find(const ptc_attn_args &a, int group, const int *pre, int u) {
+__device__ AttnItem attn_find(const ptc_attn_args &a, Group group, const int *pre, int u) {
     AttnItem it;
     const int heads = a.cache.n_kv_heads;
     int lo = 0, hi = a.n_seqs;   // last r with pre[r] * heads <= u (sequences without units share their start)
@@ -164,7 +177,7 @@ __device__ AttnItem attn_find(const ptc_attn_args &a, int group, const int *pre,
         rest -= n;
     }
     it.i0 = m * ROWS;
-    it.i1 = min(it.s.n * group, (m + 1) * ROWS);
+    it.i1 = min(it.s.n * group.n, (m + 1) * ROWS);
     attn_keys(it.s, group, a.window, it.i0, it.i1, it.lo, it.hi);
     it.first = u - rest;
     it.units = n;
@@ -210,7 +223,7 @@ __device__ __forceinline__ void cp_async_wait() {
 // out where there are few rows. All THREADS threads; smem: MT floats a part
 // and 4 a thread or 4 outputs, whichever is more.
 template <typename T, int HDP, int MT, int SLOT, int THREADS>
-__device__ void attn_merge(const ptc_attn_args &a, const AttnItem &it, int group, float *slots, int c0, int c1, float *smem) {
+__device__ void attn_merge(const ptc_attn_args &a, const AttnItem &it, Group group, float *slots, int c0, int c1, float *smem) {
                     // weights of the parts, a warp per row and a lane per part; then the
                     // weighted sum, the parts shared out where there are few rows
                     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = it.i1 - it.i0, hd = a.cache.head_dim, parts = c1 - c0 + 1;
@@ -258,8 +271,8 @@ __device__ void attn_merge(const ptc_attn_args &a, const AttnItem &it, int group
                             acc.z += v.z;
                             acc.w += v.w;
                         }
-                        const int row = it.i0 + r, tok = row / group;
-                        T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + row - tok * group) * hd + d;
+                        const int row = it.i0 + r, tok = group.div(row);
+                        T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group.n + row - tok * group.n) * hd + d;
                         dst[0] = Elem<T>::down(acc.x);
                         dst[1] = Elem<T>::down(acc.y);
                         dst[2] = Elem<T>::down(acc.z);
@@ -268,8 +281,8 @@ __device__ void attn_merge(const ptc_attn_args &a, const AttnItem &it, int group
 }
 
 // The kernel for many rows (ptc_serve_attn_wide.cu): 16-bit types, scale > 0.
-cudaError_t launch_attn_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s);
+cudaError_t launch_attn_wide(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s);
 // The one for many rows of f32 (ptc_serve_attn_f32.cu).
-cudaError_t launch_attn_f32(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s);
+cudaError_t launch_attn_f32(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s);
 
 }  // namespace ptc

@@ -26,7 +26,7 @@ struct F32Shape {
 };
 
 template <int HDP>
-__global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, int group) {
+__global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, Group group) {
     using S = F32Shape<HDP>;
     constexpr int E = HDP / 32;   // pairs of outputs of a thread and row
     extern __shared__ __align__(16) float fa_smem[];
@@ -80,9 +80,9 @@ __global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, int gr
         look(1);
         __syncthreads();
         for (int x = tid; x < FA_ROWS * (HDP / 4); x += FA_THREADS) {
-            const int r = x / (HDP / 4), d = x % (HDP / 4) * 4, row = it.i0 + r, tok = row / group;
+            const int r = x / (HDP / 4), d = x % (HDP / 4) * 4, row = it.i0 + r, tok = group.div(row);
             const bool real = r < rows && d < hd;
-            const long long off = real ? (it.s.q0 + tok) * a.q_stride + (long long)(it.head * group + row - tok * group) * hd + d : 0;
+            const long long off = real ? (it.s.q0 + tok) * a.q_stride + (long long)(it.head * group.n + row - tok * group.n) * hd + d : 0;
             cp_async16_or_zero(smem_u32(qs + r * S::ROW + d), (const float *)a.q + off, real);
         }
         fill(0);
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, int gr
         int lo[4], hi[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = ty * 4 + i, pos = it.s.pos0 + (it.i0 + r) / group;
+            const int r = ty * 4 + i, pos = it.s.pos0 + group.div(it.i0 + r);
             hi[i] = r < rows ? min(pos + 1, it.s.cap) : 0;
             lo[i] = a.window > 0 ? pos - a.window + 1 : 0;
             m[i] = -INFINITY;
@@ -175,12 +175,12 @@ __global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, int gr
         float *slot = slots + (long long)(2 * c + (seg0 == 0)) * S::SLOT;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int r = ty * 4 + i, row = it.i0 + r, tok = row / group;
+            const int r = ty * 4 + i, row = it.i0 + r, tok = group.div(row);
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
             if (r >= rows) continue;
             const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
-            float *dst = whole ? (float *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + row - tok * group) * hd : slot + r * HDP;
+            float *dst = whole ? (float *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group.n + row - tok * group.n) * hd : slot + r * HDP;
 #pragma unroll
             for (int e = 0; e < E; e++)
                 if (32 * e + 2 * tx < hd) *(float2 *)(dst + 32 * e + 2 * tx) = whole ? make_float2(o[i][e][0] * inv, o[i][e][1] * inv) : make_float2(o[i][e][0], o[i][e][1]);
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(FA_THREADS) k_attn_f32(ptc_attn_args a, int gr
 }
 
 template <int HDP>
-static cudaError_t launch(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+static cudaError_t launch(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     using S = F32Shape<HDP>;
     static_assert(FA_ROWS * FA_MAX_CTAS + 3 + FA_ROWS * HDP <= S::FLOATS, "a merge fits the tiles");
     static_assert(FA_MAX_CTAS * 2 * (long long)S::SLOT * 4 + ATTN_FLAG_BYTES <= (long long)PTC_ATTN_WORKSPACE_BYTES, "two slots for each CTA");
@@ -218,7 +218,7 @@ static cudaError_t launch(const ptc_attn_args &a, int group, int n_sm, cudaStrea
     return cudaGetLastError();
 }
 
-cudaError_t launch_attn_f32(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+cudaError_t launch_attn_f32(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     return a.cache.head_dim <= 64 ? launch<64>(a, group, n_sm, s) : launch<128>(a, group, n_sm, s);
 }
 

@@ -160,6 +160,7 @@ struct WideShared {
     unsigned tmem;
     int gave_up;
     int last;
+    float weight[8][WA_ROWS];   // of a merge
     long long scratch[WA_THREADS / 32];
 };
 
@@ -233,7 +234,7 @@ __device__ __forceinline__ void tma_box(unsigned dst, const CUtensorMap *map, in
 // The loading warps of one kind (K with Q, or V): WARPS of them, of which this
 // is the w-th. A lane looks up the cells of every 32nd key of its warp's share.
 template <typename T, int HDP, int WARPS, bool KEYS>
-__device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int run, int group, const int *pre, int u0, int u1, WideShared &sh, unsigned q_at, unsigned at, int w,
+__device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int run, Group group, const int *pre, int u0, int u1, WideShared &sh, unsigned q_at, unsigned at, int w,
                            const Waiter &wait) {
     using S = WideShape<HDP>;
     constexpr int CH = HDP / 8, SHARE = WA_KEYS / WARPS, LOOKS = SHARE / 32;
@@ -247,17 +248,6 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
         const int seg0 = u - it.first, tiles = min(it.units - seg0, u1 - u);
         const int *table = a.page_table + (long long)it.r * a.max_pages;
         const long long head = it.head * a.cache.head_stride;
-        if (KEYS) {
-            over.done<0>();   // the last S of the item before needs its K tile
-            if (items > 0) wait(&sh.bar.q_empty, (items - 1) & 1);
-            for (int x = w * 32 + lane; x < WA_ROWS * CH; x += WARPS * 32) {
-                const int row = x / CH, ch = x % CH, i = it.i0 + row, tok = i / group;
-                const bool real = i < it.i1 && ch * 8 < hd;
-                const long long off = real ? (it.s.q0 + tok) * a.q_stride + (long long)(it.head * group + i - tok * group) * hd + ch * 8 : 0;
-                cp_async16_or_zero(q_at + (row >> 7) * (S::Q / 2) + swizzled(WA_TILE, row & 127, ch), (const T *)a.q + off, real);
-            }
-            over.issued(&sh.bar.q_full);
-        }
         // a lane's run of tokens of a tile: its page, looked up one tile ahead
         const int key = w * SHARE + lane * run;
         const bool runs = run && lane * run < SHARE;
@@ -266,6 +256,21 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
             return runs && j < tiles && t < it.hi && t + run > it.lo ? table[t / a.cache.page_size] : -1;
         };
         int page = look(0);
+        if (KEYS) {
+            over.done<0>();   // the last S of the item before needs its K tile
+            if (items > 0) wait(&sh.bar.q_empty, (items - 1) & 1);
+            // a lane has one chunk of every RATE-th row
+            constexpr int RATE = WARPS * 32 / CH;
+            const int ch = (w * 32 + lane) % CH;
+#pragma unroll 4
+            for (int row = (w * 32 + lane) / CH; row < WA_ROWS; row += RATE) {
+                const int i = it.i0 + row, tok = group.div(i);
+                const bool real = i < it.i1 && ch * 8 < hd;
+                const long long off = real ? (it.s.q0 + tok) * a.q_stride + (long long)(it.head * group.n + i - tok * group.n) * hd + ch * 8 : 0;
+                cp_async16_or_zero(q_at + (row >> 7) * (S::Q / 2) + swizzled(WA_TILE, row & 127, ch), (const T *)a.q + off, real);
+            }
+            over.issued(&sh.bar.q_full);
+        }
         for (int j = 0; j < tiles; j++, n++) {
             const int s = n & 1, first = (it.lo / WA_KEYS + seg0 + j) * WA_KEYS, mine = page;
             const unsigned stage = at + s * S::KV;
@@ -377,7 +382,7 @@ __device__ void load_tiles(const ptc_attn_args &a, const CUtensorMap *map, int r
 }
 
 template <typename T, int HDP>
-__global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, const __grid_constant__ WideMaps maps, int group) {
+__global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, const __grid_constant__ WideMaps maps, Group group) {
     using S = WideShape<HDP>;
     extern __shared__ char wa_raw[];
     __shared__ WideShared sh;
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
             const AttnItem it = attn_find<WA_ROWS, WA_KEYS>(a, group, pre, u);
             const int seg0 = u - it.first, tiles = min(it.units - seg0, u1 - u), rows = it.i1 - it.i0;
             const bool active = t * WA_TILE < rows;   // of the tile, the same for its four warps
-            const int i = it.i0 + t * WA_TILE + row, tok = i / group;
+            const int i = it.i0 + t * WA_TILE + row, tok = group.div(i);
             const bool real = i < it.i1;
             // rows that are not there see everything: their zeros need no masking
             const int pos = it.s.pos0 + tok, hi = real ? min(pos + 1, it.s.cap) : INT_MAX, lo = real && a.window > 0 ? pos - a.window + 1 : 0;
@@ -618,7 +623,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
             float *slot = slots + (long long)(2 * c + (seg0 == 0)) * S::SLOT;
             if (active) {
                 const float inv = l > 0.f ? 1.f / l : 0.f;
-                T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group + i - tok * group) * hd;
+                T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group.n + i - tok * group.n) * hd;
                 float *part = slot + (t * WA_TILE + row) * HDP;
 #pragma unroll 1
                 for (int d = 0; d < HDP; d += 32) {
@@ -657,34 +662,63 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                 }
                 bar_sync(1, WA_ROWS);
                 if (sh.last) {
-                    for (int x = tid; x < rows * (HDP / 8); x += WA_ROWS) {
-                        const int r = x / (HDP / 8), d = x % (HDP / 8) * 8;
-                        if (d >= hd) continue;
-                        float top = -INFINITY, sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                        for (int p = c0; p <= c1; p++) top = fmaxf(top, __ldcg(slots + (long long)(2 * p + (p == c0)) * S::SLOT + WA_ROWS * HDP + r));
+                    // Weights of up to 8 parts at a time, a thread per row, then the weighted sums: thread x has
+                    // 8 outputs of 4 rows at once, so that the loads of a part are under way together.
+                    float top = -INFINITY, sum = 0.f;
+                    auto part = [&](int p) { return slots + (long long)(2 * p + (p == c0)) * S::SLOT; };
+                    if (tid < rows) {
+#pragma unroll 4
+                        for (int p = c0; p <= c1; p++) top = fmaxf(top, __ldcg(part(p) + WA_ROWS * HDP + tid));
                         const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 2
-                        for (int p = c0; p <= c1; p++) {
-                            const float *from = slots + (long long)(2 * p + (p == c0)) * S::SLOT;
-                            const float f = exp2f(__ldcg(from + WA_ROWS * HDP + r) - ref);
-                            sum += f * __ldcg(from + WA_ROWS * (HDP + 1) + r);
+#pragma unroll 4
+                        for (int p = c0; p <= c1; p++) sum += exp2f(__ldcg(part(p) + WA_ROWS * HDP + tid) - ref) * __ldcg(part(p) + WA_ROWS * (HDP + 1) + tid);
+                    }
+                    const float norm = (sum > 0.f ? 1.f / sum : 0.f), ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 1
+                    for (int x0 = 0; x0 < rows * (HDP / 8); x0 += 4 * WA_ROWS) {
+                        float acc[4][8];
 #pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                const float4 v = __ldcg((const float4 *)(from + r * HDP + d) + h);
-                                acc[4 * h] += f * v.x;
-                                acc[4 * h + 1] += f * v.y;
-                                acc[4 * h + 2] += f * v.z;
-                                acc[4 * h + 3] += f * v.w;
-                            }
+                        for (int k = 0; k < 4; k++)
+#pragma unroll
+                            for (int e = 0; e < 8; e++) acc[k][e] = 0.f;
+#pragma unroll 1
+                        for (int p0 = c0; p0 <= c1; p0 += 8) {
+                            bar_sync(1, WA_ROWS);
+#pragma unroll 1
+                            for (int p = p0; p <= min(c1, p0 + 7); p++)
+                                sh.weight[p - p0][tid] = tid < rows ? exp2f(__ldcg(part(p) + WA_ROWS * HDP + tid) - ref) * norm : 0.f;
+                            bar_sync(1, WA_ROWS);
+#pragma unroll 1
+                            for (int p = p0; p <= min(c1, p0 + 7); p++)
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const int x = x0 + k * WA_ROWS + tid, r = x / (HDP / 8);
+                                    if (r >= rows) continue;
+                                    const float4 *from = (const float4 *)(part(p) + r * HDP + x % (HDP / 8) * 8);
+                                    const float f = sh.weight[p - p0][r];
+                                    const float4 v = __ldcg(from), w = __ldcg(from + 1);
+                                    acc[k][0] += f * v.x;
+                                    acc[k][1] += f * v.y;
+                                    acc[k][2] += f * v.z;
+                                    acc[k][3] += f * v.w;
+                                    acc[k][4] += f * w.x;
+                                    acc[k][5] += f * w.y;
+                                    acc[k][6] += f * w.z;
+                                    acc[k][7] += f * w.w;
+                                }
                         }
-                        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-                        const int k = it.i0 + r, tk = k / group;
-                        uint4 v;
-                        v.x = pack2(acc[0] * inv, acc[1] * inv, T());
-                        v.y = pack2(acc[2] * inv, acc[3] * inv, T());
-                        v.z = pack2(acc[4] * inv, acc[5] * inv, T());
-                        v.w = pack2(acc[6] * inv, acc[7] * inv, T());
-                        *(uint4 *)((T *)a.out + (it.s.q0 + tk) * a.out_stride + (long long)(it.head * group + k - tk * group) * hd + d) = v;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int x = x0 + k * WA_ROWS + tid, r = x / (HDP / 8), d = x % (HDP / 8) * 8;
+                            if (r >= rows || d >= hd) continue;
+                            const int i2 = it.i0 + r, tk = group.div(i2);
+                            uint4 v;
+                            v.x = pack2(acc[k][0], acc[k][1], T());
+                            v.y = pack2(acc[k][2], acc[k][3], T());
+                            v.z = pack2(acc[k][4], acc[k][5], T());
+                            v.w = pack2(acc[k][6], acc[k][7], T());
+                            *(uint4 *)((T *)a.out + (it.s.q0 + tk) * a.out_stride + (long long)(it.head * group.n + i2 - tk * group.n) * hd + d) = v;
+                        }
                     }
                     if (tid == 0) flags[c0] = 0;
                 }
@@ -699,6 +733,22 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
     if (warp == 8) tm_free(TM_S, TM_COLS);
 }
 
+// The driver's encoder of tensor maps, looked up once (NULL: there is none).
+static decltype(&cuTensorMapEncodeTiled) tensor_map_encoder() {
+    static void *found;   // written once, with the same value by whoever comes first
+    void *fn = __atomic_load_n(&found, __ATOMIC_ACQUIRE);
+    if (!fn) {
+        cudaDriverEntryPointQueryResult how;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &how) != cudaSuccess ||
+            how != cudaDriverEntryPointSuccess || !fn) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        __atomic_store_n(&found, fn, __ATOMIC_RELEASE);
+    }
+    return (decltype(&cuTensorMapEncodeTiled))fn;
+}
+
 // The tensor maps of a cache. Where a page's tokens do not come in runs of 8, or
 // the driver does not take the strides, run stays 0 and the copies serve.
 static WideMaps wide_maps(const ptc_paged_cache &c) {
@@ -707,14 +757,8 @@ static WideMaps wide_maps(const ptc_paged_cache &c) {
     int run = 64;
     while (c.page_size % run) run /= 2;
     if (run < 8) return m;
-    void *fn = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess || !fn) {
-        cudaGetLastError();
-        return m;
-    }
-    const auto encode = (decltype(&cuTensorMapEncodeTiled))fn;
+    const auto encode = tensor_map_encoder();
+    if (!encode) return m;
     const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.n_kv_heads, (cuuint64_t)c.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)c.token_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)run, 1, 1}, step[4] = {1, 1, 1, 1};
@@ -728,7 +772,7 @@ static WideMaps wide_maps(const ptc_paged_cache &c) {
 }
 
 template <typename T, int HDP>
-static cudaError_t launch_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+static cudaError_t launch_wide(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     using S = WideShape<HDP>;
     static_assert(2 * 148 * (long long)S::SLOT * 4 + ATTN_FLAG_BYTES <= (long long)PTC_ATTN_WORKSPACE_BYTES, "two slots for each SM");
     auto kernel = k_attn_wide<T, HDP>;
@@ -740,7 +784,7 @@ static cudaError_t launch_wide(const ptc_attn_args &a, int group, int n_sm, cuda
     return cudaGetLastError();
 }
 
-cudaError_t launch_attn_wide(const ptc_attn_args &a, int group, int n_sm, cudaStream_t s) {
+cudaError_t launch_attn_wide(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     const bool small = a.cache.head_dim <= 64;
     if (a.cache.dtype == PTC_F16) return small ? launch_wide<__half, 64>(a, group, n_sm, s) : launch_wide<__half, 128>(a, group, n_sm, s);
     return small ? launch_wide<__nv_bfloat16, 64>(a, group, n_sm, s) : launch_wide<__nv_bfloat16, 128>(a, group, n_sm, s);
