@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                 bar_sync(1, WA_ROWS);
                 if (sh.last) {
                     // Weights of up to 8 parts at a time, a thread per row, then the weighted sums: thread x has
-                    // 8 outputs of 4 rows at once, so that the loads of a part are under way together.
+                    // 8 outputs of 8 rows at once, so that the loads of a part are under way together.
                     float top = -INFINITY, sum = 0.f;
                     auto part = [&](int p) { return slots + (long long)(2 * p + (p == c0)) * S::SLOT; };
                     if (tid < rows) {
@@ -675,23 +675,23 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                     }
                     const float norm = (sum > 0.f ? 1.f / sum : 0.f), ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 1
-                    for (int x0 = 0; x0 < rows * (HDP / 8); x0 += 4 * WA_ROWS) {
-                        float acc[4][8];
+                    for (int x0 = 0; x0 < rows * (HDP / 8); x0 += 8 * WA_ROWS) {
+                        float acc[8][8];
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
+                        for (int k = 0; k < 8; k++)
 #pragma unroll
                             for (int e = 0; e < 8; e++) acc[k][e] = 0.f;
 #pragma unroll 1
                         for (int p0 = c0; p0 <= c1; p0 += 8) {
                             bar_sync(1, WA_ROWS);
-#pragma unroll 1
+#pragma unroll 4
                             for (int p = p0; p <= min(c1, p0 + 7); p++)
                                 sh.weight[p - p0][tid] = tid < rows ? exp2f(__ldcg(part(p) + WA_ROWS * HDP + tid) - ref) * norm : 0.f;
                             bar_sync(1, WA_ROWS);
 #pragma unroll 1
                             for (int p = p0; p <= min(c1, p0 + 7); p++)
 #pragma unroll
-                                for (int k = 0; k < 4; k++) {
+                                for (int k = 0; k < 8; k++) {
                                     const int x = x0 + k * WA_ROWS + tid, r = x / (HDP / 8);
                                     if (r >= rows) continue;
                                     const float4 *from = (const float4 *)(part(p) + r * HDP + x % (HDP / 8) * 8);
@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                                 }
                         }
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
+                        for (int k = 0; k < 8; k++) {
                             const int x = x0 + k * WA_ROWS + tid, r = x / (HDP / 8), d = x % (HDP / 8) * 8;
                             if (r >= rows || d >= hd) continue;
                             const int i2 = it.i0 + r, tk = group.div(i2);
