@@ -5,11 +5,11 @@
 // kept tokens are those at or above one threshold in the order (value, lowest
 // index first), which is found by counting.
 //
-// Few kept (top_k up to 512): each thread's maximum is known from the load,
-// and the bin in which k of these maxima lie is low enough to hold the k
-// largest of all, and little more. One comparison per logit collects them (a
-// few hundred) in one CTA, which ranks them against each other for all the
-// rules.
+// Few kept (top_k up to 400): the load leaves the maxima of 512 groups of the
+// row. The bin of equal width in which k of them lie bounds the k largest
+// logits from below, and one comparison per logit collects what is above it
+// (about 512 ln(512 / (512 - k)) of logits in random order) in one CTA, which
+// ranks them against each other for all the rules.
 //
 // Otherwise:
 //  1. top_k: a histogram of the logits by their distance from the maximum
@@ -43,25 +43,30 @@ constexpr int SP_THREADS = 512;
 constexpr int SP_WARPS = SP_THREADS / 32;
 constexpr int SP_BINS = 2048;
 constexpr int SP_LIST = 1024;     // members that are ranked
-constexpr int SP_FEW = 512;       // top_k up to here by the threads' maxima
+constexpr int SP_FEW = 400;       // top_k up to here by the groups' maxima
+constexpr int SP_GROUPS = 512;
 constexpr int SP_SLICE = 16384;   // logits of a CTA, while 8 of them hold the row
 constexpr float SP_RANGE = 44.f;  // weights below 2^-44 are zero
 typedef unsigned long long u64;
 // values that the CTAs of a row tell each other, a slot each
-enum { IN_BEST, IN_FIRST, IN_FEW, IN_COUNT, IN_LIST, IN_MASS, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
+enum { IN_BEST, IN_FIRST, IN_COUNT, IN_LIST, IN_MASS, IN_LIST2, IN_KEPT, IN_STEP, SP_SLOTS = IN_STEP + 2 };
 constexpr double SP_ONE = 8796093022208.0;   // 2^43
 
 struct alignas(16) SampleShared {
-    unsigned hist[3][SP_BINS];   // counts in the first, or the low, middle and high 15 bits of masses
-    struct {
-        u64 key[SP_LIST], w[SP_LIST];
-    } all;               // the members of all CTAs, with their weights
-    u64 list[SP_LIST];   // this CTA's
+    union {
+        unsigned hist[3][SP_BINS];   // counts in the first, or the low, middle and high 15 bits of masses
+        struct {
+            u64 key[SP_LIST], w[SP_LIST];
+        } all;               // the members of all CTAs, with their weights (nobody reads the histogram any more)
+    };
+    u64 list[SP_LIST];       // this CTA's
+    float most[SP_GROUPS];   // maxima of the row's groups
     double table[256];   // 2^(j/256)
     u64 in[SP_SLOTS][8];   // what each CTA of the cluster pushed here, by value and rank
     u64 part[SP_WARPS], part2[SP_WARPS];
     u64 border[2], found;
     unsigned n_list, n_few;
+    int edge;
 };
 
 __device__ __forceinline__ float key_value(u64 key) {
@@ -329,53 +334,61 @@ __device__ __forceinline__ u64 sample_goal(float u, u64 total) {
 }
 
 // All the rules on m collected logits, among them the k largest: each is
-// ranked against the others, by one CTA.
+// ranked against the others, by one CTA. A member's comparisons are shared by
+// as many threads as there are.
 __device__ void few_tokens(const ptc_sample_args &a, SampleShared &sh, const Weigh &wt, int row, int m, int k, float p, u64 least, float u) {
-    constexpr int EACH = SP_LIST / SP_THREADS;
     const int tid = threadIdx.x;
-    u64 key[EACH], w[EACH], before[EACH], kept = 0;
-    int above[EACH];
-#pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        const int i = tid + e * SP_THREADS;
-        key[e] = i < m ? sh.list[i] : 0;
-        w[e] = i < m ? wt.weight(key_value(key[e])) : 0;
-        if (i < m) sh.all.key[i] = key[e], sh.all.w[i] = w[e];
-        before[e] = above[e] = 0;
+    int lanes = SP_THREADS / m;   // threads of a member: a power of two up to a warp
+    lanes = lanes >= 32 ? 32 : lanes >= 16 ? 16 : lanes >= 8 ? 8 : lanes >= 4 ? 4 : lanes >= 2 ? 2 : 1;
+    const int per = SP_THREADS / lanes, lane = tid % lanes, rounds = (m + per - 1) / per;   // rounds: at most 2
+    for (int i = tid; i < m; i += SP_THREADS) {
+        const u64 e = sh.list[i];
+        sh.all.key[i] = e;
+        sh.all.w[i] = wt.weight(key_value(e));
     }
     __syncthreads();
-    for (int j = 0; j < m; j++) {   // members and mass before each
-        const u64 kj = sh.all.key[j], wj = sh.all.w[j];
+    u64 mass = 0, before[2], kept = 0;
+    int above[2];
 #pragma unroll
-        for (int e = 0; e < EACH; e++)
-            if (e * SP_THREADS < m && kj > key[e]) above[e]++, before[e] += wj;
+    for (int r = 0; r < 2; r++) {   // members and mass before each
+        before[r] = 0;
+        above[r] = 0;
+        if (r >= rounds) continue;
+        const int i = r * per + tid / lanes;
+        const u64 e = i < m ? sh.all.key[i] : ~0ull;
+#pragma unroll 4
+        for (int j = lane; j < m; j += lanes)
+            if (sh.all.key[j] > e) above[r]++, before[r] += sh.all.w[j];
+        for (int d = 1; d < lanes; d *= 2) {
+            above[r] += __shfl_xor_sync(0xffffffffu, above[r], d);
+            before[r] += __shfl_xor_sync(0xffffffffu, before[r], d);
+        }
+        if (i < m && lane == 0 && above[r] < k) mass += sh.all.w[i];
     }
-    u64 mass = 0;
-#pragma unroll
-    for (int e = 0; e < EACH; e++)
-        if (tid + e * SP_THREADS < m && above[e] < k) mass += w[e];
     const double want = (double)p * (double)block_add(mass, sh.part);
 #pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        const int i = tid + e * SP_THREADS;
-        if (i >= m) break;
-        const bool keep = above[e] < k && (above[e] == 0 || p > 1.0f || (double)before[e] < want) && w[e] >= least;
-        w[e] = keep ? w[e] : 0;
-        kept += w[e];
-        sh.list[i] = (u64)argmax_key_index(key[e]) << 44 | w[e];   // a weight has at most 44 bits, an index 18
+    for (int r = 0; r < 2; r++) {
+        const int i = r * per + tid / lanes;
+        if (r >= rounds || i >= m || lane > 0) continue;
+        const u64 w = sh.all.w[i];
+        const bool keep = above[r] < k && (above[r] == 0 || p > 1.0f || (double)before[r] < want) && w >= least;
+        if (keep) kept += w;
+        sh.list[i] = (u64)argmax_key_index(sh.all.key[i]) << 44 | (keep ? w : 0);   // a weight has at most 44 bits, an index 18
     }
-    const u64 total = block_add(kept, sh.part), goal = sample_goal(u, total);
+    const u64 total = block_add(kept, sh.part), goal = sample_goal(u, total), weights = (1ull << 44) - 1;
 #pragma unroll
-    for (int e = 0; e < EACH; e++) {
-        const int i = tid + e * SP_THREADS;
-        if (i >= m || !w[e]) continue;
-        const u64 mine = sh.list[i];
+    for (int r = 0; r < 2; r++) {
+        const int i = r * per + tid / lanes;
+        if (r >= rounds) continue;
+        const u64 mine = i < m ? sh.list[i] : 0;
         u64 run = 0;   // the kept weights at lower indexes
-        for (int j = 0; j < m; j++) {
+#pragma unroll 4
+        for (int j = lane; j < m; j += lanes) {
             const u64 o = sh.list[j];
-            run += o < mine ? o & ((1ull << 44) - 1) : 0;
+            run += o < mine ? o & weights : 0;
         }
-        if (goal >= run && goal < run + w[e]) a.tokens[row] = (int)(mine >> 44);
+        for (int d = 1; d < lanes; d *= 2) run += __shfl_xor_sync(0xffffffffu, run, d);
+        if (i < m && lane == 0 && goal >= run && goal < run + (mine & weights)) a.tokens[row] = (int)(mine >> 44);
     }
 }
 
@@ -436,8 +449,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
         top = fmaxf(top, __uint_as_float((unsigned)sh.part[w]));
         lowest = fminf(lowest, __uint_as_float((unsigned)(sh.part[w] >> 32)));
     }
+    const bool by_k = want_k > 0 && want_k < a.vocab, few = by_k && want_k <= SP_FEW, by_p = p < 1.0f;
+    float group = most;   // the maximum of CL neighbouring threads: 512 / CL groups of this CTA
+#pragma unroll
+    for (int d = 1; d < CL; d *= 2) group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, d));
     cl.barrier_wait();
     R.push(IN_BEST, (u64)__float_as_uint(lowest) << 32 | __float_as_uint(top));
+    if (few)   // each of the CL threads tells one CTA
+        cl.map_shared_rank(sh.most, tid % CL)[rank * (SP_GROUPS / CL) + tid / CL] = group;
     cl.sync();
 #pragma unroll
     for (int q = 0; q < CL; q++) {
@@ -470,7 +489,6 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     const float reach = fmaxf((float)(SP_RANGE / c), 1e-37f), spread = fminf(top - lowest, reach);
     const Weigh wt = {top, reach, spread > 0.f ? fminf((SP_BINS - 1) / spread, 1e30f) : 1e30f, c, (double)top * c, sh.table};
     R.wt = wt;
-    const bool by_k = want_k > 0 && want_k < a.vocab, by_p = p < 1.0f;
     const double least_w = ceil((mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE);
     const u64 least = least_w > 0 ? (u64)least_w : 0;   // min_p as a weight
     const u64 best = order_key(top, 0);   // at or above every key
@@ -478,16 +496,27 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
 
     u64 sums[SampleRow<T, CL>::PER], total;
 
-    if (by_k && want_k <= SP_FEW) {
-        // The bin in which k of the threads' maxima lie: at least k logits are in it or before it.
-        if (wt.heavy(most)) atomicAdd(&sh.hist[0][wt.bin(most)], 1u);
-        cl.sync();
-        R.template gather<1>(sums);
-        const bool found = R.cross(sums, 0.0, want_k, total, IN_FEW);
-        R.clear(1);
-        if (found) {
-            const int edge = (int)sh.border[0];
-            unsigned *count = cl.map_shared_rank(&sh.n_few, 0);
+    if (few) {
+        // the bin in which k of the groups' maxima lie: every CTA counts them for itself
+        const float mine = sh.most[tid];
+        if (wt.heavy(mine)) atomicAdd(&sh.hist[0][wt.bin(mine)], 1u);
+        if (tid == 0) sh.edge = -1;
+        __syncthreads();
+        constexpr int EACH = SP_BINS / SP_THREADS;
+        const uint4 h = ((const uint4 *)sh.hist[0])[tid];
+        static_assert(EACH == 4, "a vector of bins per thread");
+        const int cnt[EACH] = {(int)h.x, (int)h.y, (int)h.z, (int)h.w};
+        int all, before = block_scan(cnt[0] + cnt[1] + cnt[2] + cnt[3], (int *)sh.part, all);
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            if (before < want_k && before + cnt[i] >= want_k) sh.edge = tid * EACH + i;
+            before += cnt[i];
+        }
+        ((uint4 *)sh.hist[0])[tid] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        const int edge = sh.edge;
+        unsigned *count = cl.map_shared_rank(&sh.n_few, 0);
+        if (edge >= 0) {
             u64 *list = cl.map_shared_rank(sh.list, 0);
             if (wt.bin(most) <= edge)
                 R.each([&](float v, int i) {
@@ -505,7 +534,6 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 return;
             }
         }
-        __syncthreads();
     }
     if (by_k) {
         R.each([&](float v, int) {
@@ -530,7 +558,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
                 floor = Floor::of(R.bisect_count(want_k, best));
             }
         }
-        R.clear(1);
+        __syncthreads();
+        R.clear(3);
         __syncthreads();
     }
     if (by_p && p > 0.0f) {
