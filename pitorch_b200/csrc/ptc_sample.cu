@@ -333,62 +333,54 @@ __device__ __forceinline__ u64 sample_goal(float u, u64 total) {
     return min(goal, total - 1);
 }
 
-// All the rules on m collected logits, among them the k largest: each is
-// ranked against the others, by one CTA. A member's comparisons are shared by
-// as many threads as there are.
+// All the rules on m collected logits, among them the k largest, by one CTA:
+// each is ranked against the others (its comparisons shared by as many threads
+// as there are), the weights are summed in the order of the ranks, and those
+// that are kept, at most k, ranked by index for the running sum.
 __device__ void few_tokens(const ptc_sample_args &a, SampleShared &sh, const Weigh &wt, int row, int m, int k, float p, u64 least, float u) {
     const int tid = threadIdx.x;
-    int lanes = SP_THREADS / m;   // threads of a member: a power of two up to a warp
-    lanes = lanes >= 32 ? 32 : lanes >= 16 ? 16 : lanes >= 8 ? 8 : lanes >= 4 ? 4 : lanes >= 2 ? 2 : 1;
-    const int per = SP_THREADS / lanes, lane = tid % lanes, rounds = (m + per - 1) / per;   // rounds: at most 2
-    for (int i = tid; i < m; i += SP_THREADS) {
-        const u64 e = sh.list[i];
-        sh.all.key[i] = e;
-        sh.all.w[i] = wt.weight(key_value(e));
+    const int fit = SP_THREADS / m, lanes = fit >= 32 ? 32 : fit >= 16 ? 16 : fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 1;
+    const int per = SP_THREADS / lanes, lane = tid % lanes;
+    if (tid == 0) sh.n_list = 0;
+    for (int i0 = 0; i0 < m; i0 += per) {
+        const int i = i0 + tid / lanes;
+        const u64 e = i < m ? sh.list[i] : ~0ull;
+        int rank = 0;
+#pragma unroll 4
+        for (int j = lane; j < m; j += lanes) rank += sh.list[j] > e;
+        for (int d = 1; d < lanes; d *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+        if (i < m && lane == 0) sh.all.key[rank] = e;
     }
     __syncthreads();
-    u64 mass = 0, before[2], kept = 0;
-    int above[2];
+    // in descending order, two to a thread: the weights and the sum before each
+    const int n = min(m, k);
+    u64 w[2], sum, before;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {   // members and mass before each
-        before[r] = 0;
-        above[r] = 0;
-        if (r >= rounds) continue;
-        const int i = r * per + tid / lanes;
-        const u64 e = i < m ? sh.all.key[i] : ~0ull;
-#pragma unroll 4
-        for (int j = lane; j < m; j += lanes)
-            if (sh.all.key[j] > e) above[r]++, before[r] += sh.all.w[j];
-        for (int d = 1; d < lanes; d *= 2) {
-            above[r] += __shfl_xor_sync(0xffffffffu, above[r], d);
-            before[r] += __shfl_xor_sync(0xffffffffu, before[r], d);
+    for (int e = 0; e < 2; e++) w[e] = 2 * tid + e < n ? wt.weight(key_value(sh.all.key[2 * tid + e])) : 0;
+    before = block_scan(w[0] + w[1], sh.part, sum);
+    const double want = (double)p * (double)sum;
+    u64 kept = 0;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const int i = 2 * tid + e;
+        if (i < n && (i == 0 || p > 1.0f || (double)before < want) && w[e] >= least && w[e]) {
+            kept += w[e];
+            // a weight has at most 44 bits, an index 18
+            sh.all.w[atomicAdd(&sh.n_list, 1u)] = (u64)argmax_key_index(sh.all.key[i]) << 44 | w[e];
         }
-        if (i < m && lane == 0 && above[r] < k) mass += sh.all.w[i];
-    }
-    const double want = (double)p * (double)block_add(mass, sh.part);
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int i = r * per + tid / lanes;
-        if (r >= rounds || i >= m || lane > 0) continue;
-        const u64 w = sh.all.w[i];
-        const bool keep = above[r] < k && (above[r] == 0 || p > 1.0f || (double)before[r] < want) && w >= least;
-        if (keep) kept += w;
-        sh.list[i] = (u64)argmax_key_index(sh.all.key[i]) << 44 | (keep ? w : 0);   // a weight has at most 44 bits, an index 18
+        before += w[e];
     }
     const u64 total = block_add(kept, sh.part), goal = sample_goal(u, total), weights = (1ull << 44) - 1;
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-        const int i = r * per + tid / lanes;
-        if (r >= rounds) continue;
-        const u64 mine = i < m ? sh.list[i] : 0;
+    const int q = (int)sh.n_list;
+    for (int i = tid; i < q; i += SP_THREADS) {
+        const u64 mine = sh.all.w[i];
         u64 run = 0;   // the kept weights at lower indexes
 #pragma unroll 4
-        for (int j = lane; j < m; j += lanes) {
-            const u64 o = sh.list[j];
+        for (int j = 0; j < q; j++) {
+            const u64 o = sh.all.w[j];
             run += o < mine ? o & weights : 0;
         }
-        for (int d = 1; d < lanes; d *= 2) run += __shfl_xor_sync(0xffffffffu, run, d);
-        if (i < m && lane == 0 && goal >= run && goal < run + (mine & weights)) a.tokens[row] = (int)(mine >> 44);
+        if (goal >= run && goal < run + (mine & weights)) a.tokens[row] = (int)(mine >> 44);
     }
 }
 
