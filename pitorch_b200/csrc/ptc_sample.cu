@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
 
 // CTAs per row: as many as give the batch one CTA for every place on the GPU
 // (two per SM), so that a few rows are spread and many are not, but enough
-// that a slice fits. Measured at 32000 logits: TODO.
+// that a slice fits.
 static int sample_cluster(int rows, int vocab, int n_sm) {
     int c = 1;
     while (c < 8 && ((long long)rows * c * 2 <= 2 * n_sm || vocab > c * SP_SLICE)) c *= 2;

@@ -101,15 +101,17 @@ struct NarrowRows {
     __device__ void step(unsigned at, const char *, int key, unsigned there, float scale, const float *, float *) {
         using S = NarrowShape<T, HDP, MT>;
         const int lane = threadIdx.x & 31;
-        float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        float s[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, s2[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};   // two chains of products
         const unsigned kat = at + ((lane & 7) + ((lane >> 4) << 3)) * S::ROW + ((lane >> 3) & 1) * 16;
 #pragma unroll
         for (int k = 0; k < HDP / 16; k++) {
             uint32_t b[4];
             ldmatrix4(b, kat + k * 32);
-            mma16816(s[0], q[k], b[0], b[1], T());
-            mma16816(s[1], q[k], b[2], b[3], T());
+            mma16816(k & 1 ? s2[0] : s[0], q[k], b[0], b[1], T());
+            mma16816(k & 1 ? s2[1] : s[1], q[k], b[2], b[3], T());
         }
+#pragma unroll
+        for (int x = 0; x < 8; x++) s[x >> 2][x & 3] += s2[x >> 2][x & 3];
         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -148,19 +150,26 @@ struct NarrowRows {
                     l[h] += v;
                 }
         }
-        // probabilities rounded to the type for the product with V, as one operand type has to be (their sum is not)
-        const uint32_t p[4] = {pack2(s[0][0], s[0][1], T()), pack2(s[0][2], s[0][3], T()), pack2(s[1][0], s[1][1], T()),
-                               pack2(s[1][2], s[1][3], T())};
+        // The product with V wants probabilities of V's type: rounded, and what the rounding left, as a second product
+        // (rounded alone they would add as large an error as the result's own rounding).
+        uint32_t p[4], rest[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            float &u = s[x >> 1][2 * (x & 1)], &w = s[x >> 1][2 * (x & 1) + 1];
+            p[x] = pack2(u, w, T());
+            const T *r = (const T *)&p[x];
+            rest[x] = pack2(u - Elem<T>::up(r[0]), w - Elem<T>::up(r[1]), T());
+        }
         const unsigned vat = at + NA_KEYS * S::ROW + (lane & 15) * S::ROW + (lane >> 4) * 16;
 #pragma unroll
-        for (int n = 0; n < HDP / 16; n++) {
-            uint32_t b[4];
-            ldmatrix4t(b, vat + n * 32);
+        for (int n = 0; n < HDP / 16; n += 2) {   // two at a time: the second products follow the first at a distance
+            uint32_t b[2][4];
+            ldmatrix4t(b[0], vat + n * 32);
+            ldmatrix4t(b[1], vat + n * 32 + 32);
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                float(&c)[4] = o[2 * n + x];
-                mma16816(c, p, b[2 * x], b[2 * x + 1], T());
-            }
+            for (int x = 0; x < 4; x++) mma16816(o[2 * n + x], p, b[x >> 1][2 * (x & 1)], b[x >> 1][2 * (x & 1) + 1], T());
+#pragma unroll
+            for (int x = 0; x < 4; x++) mma16816(o[2 * n + x], rest, b[x >> 1][2 * (x & 1)], b[x >> 1][2 * (x & 1) + 1], T());
         }
     }
 
@@ -317,15 +326,31 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, Gro
             const unsigned there = __ballot_sync(0xffffffffu, cell >= 0) & 0xffffu;
             if (j < n) {
                 const unsigned at = smem_u32(ring + (j % NA_STAGES) * S::STAGE);
+                const long long cell0 = __shfl_sync(0xffffffffu, cell, 0);
+                if (32 % S::CH == 0 && __all_sync(0xffffffffu, cell >= 0 && cell == cell0 + (lane & 15) * a.cache.token_stride)) {
+                    // all there and one after the other, as in a page: no lane has to ask another for its key
+                    constexpr int EACH = 32 / (S::CH <= 32 ? S::CH : 32);   // keys of a step
+                    const int k0 = lane / S::CH, ch = lane % S::CH, e = ch * (16 / (int)sizeof(T));
+                    const bool real = e < hd;
+                    const long long off = cell0 + base + k0 * a.cache.token_stride + (real ? e : 0), step = EACH * a.cache.token_stride;
+                    const T *k = (const T *)a.cache.k + off, *v = (const T *)a.cache.v + off;
+                    const unsigned to = at + k0 * S::ROW + ch * 16;
 #pragma unroll
-                for (int i = 0; i < NA_KEYS * S::CH / 32; i++) {
-                    const int x = i * 32 + lane, k = x / S::CH, ch = x % S::CH;
-                    const long long from = __shfl_sync(0xffffffffu, cell, k);
-                    const int e = ch * (16 / (int)sizeof(T));
-                    const bool real = from >= 0 && e < hd;
-                    const long long off = real ? from + base + e : 0;
-                    cp_async16_or_zero(at + k * S::ROW + ch * 16, (const T *)a.cache.k + off, real);
-                    cp_async16_or_zero(at + (NA_KEYS + k) * S::ROW + ch * 16, (const T *)a.cache.v + off, real);
+                    for (int i = 0; i < NA_KEYS / EACH; i++, k += step, v += step) {
+                        cp_async16_or_zero(to + i * EACH * S::ROW, k, real);
+                        cp_async16_or_zero(to + (NA_KEYS + i * EACH) * S::ROW, v, real);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NA_KEYS * S::CH / 32; i++) {
+                        const int x = i * 32 + lane, k = x / S::CH, ch = x % S::CH;
+                        const long long from = __shfl_sync(0xffffffffu, cell, k);
+                        const int e = ch * (16 / (int)sizeof(T));
+                        const bool real = from >= 0 && e < hd;
+                        const long long off = real ? from + base + e : 0;
+                        cp_async16_or_zero(at + k * S::ROW + ch * 16, (const T *)a.cache.k + off, real);
+                        cp_async16_or_zero(at + (NA_KEYS + k) * S::ROW + ch * 16, (const T *)a.cache.v + off, real);
+                    }
                 }
             }
             cp_async_commit();
