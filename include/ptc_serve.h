@@ -156,10 +156,13 @@ int ptc_rope_table(float *table, int n_pos, int head_dim, void *stream);
  * knows it: it selects the kernel, not the result. Rows of q and out beyond
  * q_start[n_seqs] are neither read nor written. q_start has to rise from 0 to
  * at most n_tokens (LENGTH, the sequence is left out), kv_len may not pass
- * max_pages * page_size (LENGTH, positions behind it are left out), and
+ * max_pages * page_size or 2^30 (LENGTH, positions behind it are left out), and
  * positions of pages outside [0, n_pages) are left out too (INDEX).
  * q and out have the cache's type; strides in elements, multiples of 16
- * bytes. The same inputs give the same bits in every call. */
+ * bytes; n_tokens * n_heads at most 2^30. What lies behind a sequence's last
+ * position may be anything, NaN included; its own cached values should be
+ * finite, as one that is not can reach rows of that sequence which do not see
+ * its position. The same inputs give the same bits in every call. */
 typedef struct {
     ptc_paged_cache cache;
     int n_seqs;             /* 0 .. PTC_SERVE_MAX_SEQS */

@@ -490,7 +490,7 @@ static cudaError_t launch_narrow_hd(const ptc_attn_args &a, Group group, int n_s
 
 extern "C" int ptc_paged_attention(const ptc_attn_args *p, void *stream) {
     if (!p) SERVE_REFUSE("no arguments");
-    const ptc_attn_args a = *p;
+    ptc_attn_args a = *p;
     if (const char *why = ptc::check_cache(a.cache)) SERVE_REFUSE("%s", why);
     if (a.n_seqs < 0 || a.n_tokens < 0 || a.max_pages < 1 || a.max_q < 0 || a.window < 0)
         SERVE_REFUSE("bad size (n_seqs %d, n_tokens %d, max_q %d, max_pages %d, window %d)", a.n_seqs, a.n_tokens, a.max_q,
@@ -499,7 +499,9 @@ extern "C" int ptc_paged_attention(const ptc_attn_args *p, void *stream) {
     if (a.n_heads < 1 || a.n_heads % a.cache.n_kv_heads)
         SERVE_REFUSE("n_heads %d is no multiple of n_kv_heads %d", a.n_heads, a.cache.n_kv_heads);
     if (!(a.scale > -INFINITY && a.scale < INFINITY)) SERVE_REFUSE("scale is not finite");
+    if ((long long)a.n_tokens * a.n_heads > ptc::ATTN_MAX_KEYS) SERVE_REFUSE("n_tokens * n_heads passes 2^30");
     if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
+    if (a.window >= ptc::ATTN_MAX_KEYS) a.window = 0;   // it hides nothing
     const long long u = 16 / ptc::dtype_bytes(a.cache.dtype), hd = a.cache.head_dim;
     if (!a.q || !a.out || !a.page_table || !a.kv_len || !a.q_start || !a.workspace) SERVE_REFUSE("a required pointer is NULL");
     if (!ptc::aligned16(a.q) || !ptc::aligned16(a.out) || a.q_stride % u || a.out_stride % u ||

@@ -22,6 +22,7 @@
 namespace ptc {
 
 constexpr int ATTN_MAX_SEQS = PTC_SERVE_MAX_SEQS;
+constexpr int ATTN_MAX_KEYS = 1 << 30;  // positions and rows stay below it, so that sums with a tile or a window fit
 constexpr int ATTN_FLAG_BYTES = 4096;   // counters at the front of the workspace, one per CTA
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -51,7 +52,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const ptc_attn_args &a, int r) {
     AttnSeq s;
     s.q0 = a.q_start[r];
     const int q1 = a.q_start[r + 1], kv = a.kv_len[r];
-    const long long room = (long long)a.max_pages * a.cache.page_size;
+    const long long room = min((long long)a.max_pages * a.cache.page_size, (long long)ATTN_MAX_KEYS);
     s.n = q1 - s.q0;
     s.bad = 0;
     s.pos0 = kv - s.n;

@@ -54,7 +54,7 @@ BAD = ([("ptc_plan_pages", pages, kw) for kw in (
            dict(v_stride=132), dict(q_out_stride=248))]
        + [("ptc_paged_attention", attn, dict(cache=c)) for c in BAD_CACHE]
        + [("ptc_paged_attention", attn, kw) for kw in (
-           dict(n_seqs=-1), dict(n_seqs=4097), dict(n_tokens=-1), dict(n_heads=0), dict(n_heads=3), dict(max_q=-1), dict(max_pages=0), dict(window=-1),
+           dict(n_seqs=-1), dict(n_seqs=4097), dict(n_tokens=-1), dict(n_tokens=(1 << 28) + 1), dict(n_heads=0), dict(n_heads=3), dict(max_q=-1), dict(max_pages=0), dict(window=-1),
            dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(q=A + 8), dict(q_stride=248), dict(q_stride=257),
            dict(out=None), dict(out_stride=128), dict(page_table=None), dict(kv_len=None), dict(q_start=None), dict(workspace=None),
            dict(workspace=A + 16), dict(workspace_bytes=api.PTC_ATTN_WORKSPACE_BYTES - 1))]

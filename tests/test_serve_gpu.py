@@ -1,8 +1,10 @@
 """The serving operators (include/ptc_serve.h) against 64-bit plain forms:
 page tables and slot maps, the rotary cache write, paged attention, sampling."""
-import ctypes as C
 import math
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 
@@ -245,6 +247,49 @@ def test_rows_without_a_position_are_zero(ptlib, dtype):
     check(got[: b.total], want, bound)
     assert not bool(got[:3].any()) and not bool(got[5:147].any())
     assert int(b.err) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [6, 140])
+def test_largest_window_and_longest_length(ptlib, dtype, new):
+    b = Batch([(-3, new), (40, new), (20, new)], 2, 2, 32, 8, dtype)
+    want, bound = b.reference()
+    check(b.attend(ptlib, window=2 ** 31 - 1)[: b.total], want, bound)
+    assert int(b.err) == 0
+    # a length that no table holds: what the table holds is used (all of it behind the other rows' positions here)
+    b.kv_len[1] = 2 ** 31 - 1
+    got = b.attend(ptlib, window=0)
+    assert int(b.err) & api.PTC_SERVE_ERR_LENGTH
+    for r in (0, 2):
+        check(got[r * new:(r + 1) * new], want[r * new:(r + 1) * new], bound[r * new:(r + 1) * new])
+
+
+FIRST_CALL = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import pitorch_b200
+from pitorch_b200 import api
+from serve_ref import Batch, check, stream
+L = pitorch_b200.lib()
+b = Batch([(300, %d), (7, %d)], 2, 2, 64, 16, %r)
+out = torch.zeros_like(b.q)
+args = b.attn_args(out)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    assert L.ptc_paged_attention(args, stream()) == 0
+g.replay()
+torch.cuda.synchronize()
+check(out[: b.total], *b.reference())
+"""
+
+
+@pytest.mark.parametrize("dtype,new", [("f32", 1), ("f32", 60), ("bf16", 1), ("bf16", 60)])
+def test_first_call_of_a_process_may_be_captured(ptlib, dtype, new):
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = FIRST_CALL % (os.path.dirname(here), here, new, new, dtype)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
