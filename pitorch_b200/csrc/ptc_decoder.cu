@@ -64,6 +64,7 @@ struct ptc_decoder {
     cudaGraphExec_t g_host, g_dev;
     cudaGraphExec_t g_devk;  // DEV_TOKENS device-loop tokens per launch (null: not used)
     int fetch_logits;      // ptc_decoder_enqueue_fetch copied the logits into stage
+    int logits_part;       // the last classifier was vocab-parallel: m.logits has this rank's rows of it alone
     int w2t_stale;         // the weights changed since w2t was derived (re-derived before the next decode)
     unsigned long long *trace_buf;  // phase timeline record (m.trace while tracing)
     size_t trace_n;        // its entries
@@ -411,6 +412,7 @@ static void wait_next(ptc_decoder *d) {
 extern "C" int ptc_decoder_step(ptc_decoder *d, int token, int pos, float *logits_host) {
     if (pos < 0 || pos >= d->m.seq) PTC_FATAL("decode position %d outside [0, %d)", pos, d->m.seq);
     refresh_derived(d);
+    d->logits_part = 0;
     if (d->has_embed && (token < 0 || token >= d->m.V))
         PTC_FATAL("token %d outside [0, %d)", token, d->m.V);
     set_mode(d, 0);
@@ -478,6 +480,7 @@ extern "C" void ptc_decoder_generate_begin(ptc_decoder *d, const int *prompt, in
 
 extern "C" void ptc_decoder_enqueue_steps(ptc_decoder *d, int n) {
     refresh_derived(d);
+    if (n > 0) d->logits_part = 0;
     int i = 0;
     if (d->g_devk)
         for (; i + DEV_TOKENS <= n; i += DEV_TOKENS) PTC_CHECK(cudaGraphLaunch(d->g_devk, d->stream));
@@ -529,6 +532,7 @@ extern "C" void ptc_decoder_enqueue_layers(ptc_decoder *d, int pos, int l_start,
 // take a host token/position; the pipeline's device loop keeps mode 1.
 extern "C" void ptc_decoder_enqueue_head(ptc_decoder *d) {
     if (!d->has_head) PTC_FATAL("decoder has no head");
+    d->logits_part = 0;
     ptc::launch_head(d->m, d->n_sm, d->stream);
 }
 
@@ -562,8 +566,10 @@ extern "C" void ptc_decoder_enqueue_fetch(ptc_decoder *d, int logits) {
     PTC_CHECK(cudaMemcpyAsync(&d->io->next, &d->m.step->next, sizeof(int), cudaMemcpyDeviceToHost, d->stream));
     PTC_CHECK(cudaMemcpyAsync(&d->io->err, d->m.err, sizeof(int), cudaMemcpyDeviceToHost, d->stream));
     d->fetch_logits = logits && d->has_head;
-    if (d->fetch_logits)
+    if (d->fetch_logits) {
+        d->logits_part = 0;   // the caller has gathered the other ranks' rows
         PTC_CHECK(cudaMemcpyAsync(d->stage, d->m.logits, (size_t)d->m.V * 4, cudaMemcpyDeviceToHost, d->stream));
+    }
 }
 
 extern "C" int ptc_decoder_take_next(ptc_decoder *d, float *logits_host) {
@@ -589,6 +595,7 @@ extern "C" void ptc_decoder_enqueue_kernel(ptc_decoder *d, int kind, int l, int 
     put_step_int(d, &d->m.step->pos, pos);
     if (kind == 2) {
         if (!d->has_head) PTC_FATAL("decoder has no head");
+        d->logits_part = 0;
         ptc::launch_head(d->m, d->n_sm, d->stream);
         return;
     }
@@ -685,6 +692,7 @@ extern "C" void ptc_decoder_set_stop(ptc_decoder *d, int n_pos) {
 extern "C" void ptc_decoder_enqueue_stage(ptc_decoder *d, int n) {
     refresh_derived(d);
     if (!d->m.in_box) PTC_FATAL("ptc_decoder_enqueue_stage without pipeline links");
+    if (n > 0) d->logits_part = d->m.vp_rows > 0;
     int i = 0;
     for (; i + STAGE_POS <= n; i += STAGE_POS) PTC_CHECK(cudaGraphLaunch(d->g_stage, d->stream));
     for (; i < n; i++) PTC_CHECK(cudaGraphLaunch(d->g_stage1, d->stream));
@@ -802,8 +810,9 @@ extern "C" int ptc_decoder_prefill(ptc_decoder *d, const int *tokens, int n, int
 }
 
 extern "C" int ptc_decoder_sample(ptc_decoder *d, float temperature, int top_k, float top_p, float min_p, float u) {
-    if (!d->has_head) {
-        fprintf(stderr, "pitorch_b200: ptc_decoder_sample: no classifier\n");
+    const char *why = !d->has_head ? "no classifier" : d->logits_part ? "the logits are one rank's rows of a vocab-parallel classifier" : nullptr;
+    if (why) {
+        fprintf(stderr, "pitorch_b200: ptc_decoder_sample: %s\n", why);
         return -1;
     }
     PTC_CHECK(cudaSetDevice(ptc_device(d->ctx)));
