@@ -69,7 +69,7 @@ typedef struct {
     int n_seqs;             /* 0 .. PTC_SERVE_MAX_SEQS */
     int page_size;          /* tokens per page, >= 1 */
     int max_pages;          /* columns of page_table, >= 1 */
-    int max_tokens;         /* entries of slots and positions */
+    int max_tokens;         /* entries of slots and positions, at most 2^30 */
     int n_free;             /* entries of free_pages */
     int n_pages;            /* pages of the cache; n_pages * page_size < 2^31 */
     const int *past_len;    /* [n_seqs] */

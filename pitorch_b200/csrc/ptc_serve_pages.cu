@@ -31,6 +31,7 @@ const char *check_cache(const ptc_paged_cache &c) {
 // written only behind them, so no CTA reads what another writes.
 // ---------------------------------------------------------------------------
 constexpr int PLAN_THREADS = 512;
+constexpr int PLAN_MAX_TOKENS = 1 << 30;   // a row and a grid's step behind it fit 32 bits
 
 __device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((unsigned)tokens + page - 1) / (unsigned)page); }
 
@@ -209,7 +210,7 @@ extern "C" int ptc_plan_pages(const ptc_pages_args *p, void *stream) {
     if (!p) SERVE_REFUSE("no arguments");
     const ptc_pages_args a = *p;
     if (a.n_seqs < 0 || a.n_seqs > PTC_SERVE_MAX_SEQS) SERVE_REFUSE("n_seqs %d is outside 0..%d", a.n_seqs, PTC_SERVE_MAX_SEQS);
-    if (a.page_size < 1 || a.max_pages < 1 || a.max_tokens < 0 || a.n_free < 0 || a.n_pages < 1)
+    if (a.page_size < 1 || a.max_pages < 1 || a.max_tokens < 0 || a.max_tokens > ptc::PLAN_MAX_TOKENS || a.n_free < 0 || a.n_pages < 1)
         SERVE_REFUSE("bad size (page_size %d, max_pages %d, max_tokens %d, n_free %d, n_pages %d)", a.page_size,
                      a.max_pages, a.max_tokens, a.n_free, a.n_pages);
     if ((long long)a.n_pages * a.page_size > INT_MAX) SERVE_REFUSE("n_pages * page_size passes 2^31");
