@@ -56,6 +56,7 @@ PTC_F32, PTC_F16, PTC_BF16 = 0, 1, 2
 PTC_SERVE_ERR_PAGES, PTC_SERVE_ERR_TABLE, PTC_SERVE_ERR_TOKENS = 1, 2, 4
 PTC_SERVE_ERR_LENGTH, PTC_SERVE_ERR_INDEX, PTC_SERVE_ERR_WAIT = 8, 16, 32
 PTC_ATTN_WORKSPACE_BYTES = 64 << 20
+PTC_SERVE_MAX_SEQS, PTC_SAMPLE_MAX_VOCAB = 4096, 262144
 
 
 class ptc_pages_args(C.Structure):

@@ -676,11 +676,16 @@ static int sample_cluster(int rows, int vocab, int n_sm) {
     return c;
 }
 
+// Shared memory of a CTA with a slice of n logits (and the odd ends of its vectors).
+template <typename T>
+static constexpr int sample_smem(int n) {
+    return (int)(sizeof(SampleShared) + ((size_t)n * sizeof(T) + 47) / 16 * 16);
+}
+
 template <typename T, int CL>
 static cudaError_t launch_sample_cl(const ptc_sample_args &a, cudaStream_t s) {
-    const int slice = (a.vocab + CL - 1) / CL;
-    const size_t smem = sizeof(SampleShared) + ((size_t)slice * sizeof(T) + 47) / 16 * 16;   // with the odd ends
-    cudaError_t e = cudaFuncSetAttribute(k_sample<T, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const int slice = (a.vocab + CL - 1) / CL, smem = sample_smem<T>(slice);
+    cudaError_t e = allow_smem(k_sample<T, CL>, sample_smem<T>(CL < 8 ? SP_SLICE : PTC_SAMPLE_MAX_VOCAB / CL));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * CL));

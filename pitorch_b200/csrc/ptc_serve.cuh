@@ -53,6 +53,15 @@ private:
     cudaError_t err_;
 };
 
+// Lets `kernel` have `most` bytes of dynamic shared memory on the current
+// device. The limit belongs to the function, not to a call: `most` is what
+// the largest call of the kernel takes, the same in every call, as a
+// smaller one from another host thread would refuse a launch in between.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel *kernel, int most) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+}
+
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 inline int dtype_bytes(int dtype) { return dtype == PTC_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == PTC_F32 || dtype == PTC_F16 || dtype == PTC_BF16; }

@@ -458,12 +458,13 @@ __global__ void __launch_bounds__(NA_THREADS) k_attn_narrow(ptc_attn_args a, Gro
 template <typename T, int HDP, int MT>
 static cudaError_t launch_narrow(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {
     auto kernel = k_attn_narrow<T, HDP, MT>;
-    const int smem = NA_WARPS * NarrowShape<T, HDP, MT>::WARP + (a.n_seqs + 1) * (int)sizeof(int);
+    constexpr int ring = NA_WARPS * NarrowShape<T, HDP, MT>::WARP;
+    const int smem = attn_smem(ring, a.n_seqs);
     static_assert(NA_WARPS * MT * HDP * 4 <= NA_WARPS * NarrowShape<T, HDP, MT>::WARP, "the outputs fit the stages");
     // (and so do a merge's weights and sums: MT a part, of at most the CTAs, and 4 floats a thread or an output)
     static_assert((MT * NA_MAX_CTAS + 3) * 4 + 4 * (NA_THREADS > MT * HDP / 4 ? NA_THREADS : MT * HDP / 4) * 4 <=
                       NA_WARPS * NarrowShape<T, HDP, MT>::WARP, "a merge fits the stages");
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = allow_smem(kernel, attn_smem(ring, ATTN_MAX_SEQS));
     int per = 0;
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, NA_THREADS, smem);
     if (e != cudaSuccess) return e;

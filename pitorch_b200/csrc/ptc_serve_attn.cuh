@@ -22,6 +22,8 @@
 namespace ptc {
 
 constexpr int ATTN_MAX_SEQS = PTC_SERVE_MAX_SEQS;
+// Dynamic shared memory of a kernel behind `bytes` of its own: the sequences' first units (attn_prefix).
+constexpr int attn_smem(int bytes, int n_seqs) { return bytes + (n_seqs + 1) * (int)sizeof(int); }
 constexpr int ATTN_MAX_KEYS = 1 << 30;  // positions and rows stay below it, so that sums with a tile or a window fit
 constexpr int ATTN_FLAG_BYTES = 4096;   // counters at the front of the workspace, one per CTA
 constexpr float LOG2E = 1.4426950408889634f;

@@ -209,8 +209,8 @@ static cudaError_t launch(const ptc_attn_args &a, Group group, int n_sm, cudaStr
     static_assert(FA_ROWS * FA_MAX_CTAS + 3 + FA_ROWS * HDP <= S::FLOATS, "a merge fits the tiles");
     static_assert(FA_MAX_CTAS * 2 * (long long)S::SLOT * 4 + ATTN_FLAG_BYTES <= (long long)PTC_ATTN_WORKSPACE_BYTES, "two slots for each CTA");
     auto kernel = k_attn_f32<HDP>;
-    const int smem = S::FLOATS * 4 + (a.n_seqs + 1) * (int)sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const int smem = attn_smem(S::FLOATS * 4, a.n_seqs);
+    cudaError_t e = allow_smem(kernel, attn_smem(S::FLOATS * 4, ATTN_MAX_SEQS));
     int per = 0;
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, FA_THREADS, smem);
     if (e != cudaSuccess) return e;

@@ -798,8 +798,8 @@ static cudaError_t launch_wide(const ptc_attn_args &a, Group group, int n_sm, cu
     using S = WideShape<HDP>;
     static_assert(2 * 148 * (long long)S::SLOT * 4 + ATTN_FLAG_BYTES <= (long long)PTC_ATTN_WORKSPACE_BYTES, "two slots for each SM");
     auto kernel = k_attn_wide<T, HDP>;
-    const int smem = 1024 + S::BYTES + (a.n_seqs + 1) * (int)sizeof(int);
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const int smem = attn_smem(1024 + S::BYTES, a.n_seqs);
+    const cudaError_t e = allow_smem(kernel, attn_smem(1024 + S::BYTES, ATTN_MAX_SEQS));
     if (e != cudaSuccess) return e;
     const long long fit = (long long)(PTC_ATTN_WORKSPACE_BYTES - ATTN_FLAG_BYTES) / (2 * S::SLOT * (int)sizeof(float));
     kernel<<<(unsigned)(n_sm < fit ? n_sm : fit), WA_THREADS, smem, s>>>(a, wide_maps(a.cache), group);
