@@ -1766,8 +1766,11 @@ __global__ void k_rope_table(float2 *t, int seq, int hd) {
 
 cudaError_t launch_rope_table(float2 *t, int seq, int hd, cudaStream_t s) {
     const int n = seq * (hd / 2);
-    k_rope_table<<<(n + 255) / 256, 256, 0, s>>>(t, seq, hd);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};   // (its return value is this launch's error, never an older one)
+    cfg.gridDim = dim3((n + 255) / 256);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, k_rope_table, t, seq, hd);
 }
 
 void build_rope_table(float2 *t, int seq, int hd, cudaStream_t s) { PTC_CHECK(launch_rope_table(t, seq, hd, s)); }

@@ -20,10 +20,15 @@
         return -1;                                           \
     } while (0)
 
-#define SERVE_CUDA(call)                                                                    \
-    do {                                                                                    \
-        cudaError_t e_ = (call);                                                            \
-        if (e_ != cudaSuccess) SERVE_REFUSE("%s: %s", #call, cudaGetErrorString(e_));       \
+// The runtime also remembers a call's error for whoever asks for the last one:
+// it is taken back, as it is this call's and told by its return value.
+#define SERVE_CUDA(call)                                              \
+    do {                                                              \
+        cudaError_t e_ = (call);                                      \
+        if (e_ != cudaSuccess) {                                      \
+            cudaGetLastError();                                       \
+            SERVE_REFUSE("%s: %s", #call, cudaGetErrorString(e_));    \
+        }                                                             \
     } while (0)
 
 namespace ptc {
@@ -60,6 +65,19 @@ private:
 template <typename Kernel>
 cudaError_t allow_smem(Kernel *kernel, int most) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+}
+
+// A launch that answers for itself: the last error, which <<<>>> leaves to ask
+// for, may be an older one of the calling thread, and the call would be
+// refused although its kernel runs.
+template <typename... P, typename... A>
+cudaError_t launch_kernel(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }

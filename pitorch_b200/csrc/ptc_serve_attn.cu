@@ -474,8 +474,7 @@ static cudaError_t launch_narrow(const ptc_attn_args &a, Group group, int n_sm, 
     if (grid > fit) grid = (int)fit;
     if (grid > NA_MAX_CTAS) grid = NA_MAX_CTAS;
     static_assert(NA_MAX_CTAS <= ATTN_FLAG_BYTES / 4, "a counter per CTA");
-    kernel<<<grid, NA_THREADS, smem, s>>>(a, group);
-    return cudaGetLastError();
+    return launch_kernel(kernel, grid, NA_THREADS, smem, s, a, group);
 }
 
 template <typename T, int MT>

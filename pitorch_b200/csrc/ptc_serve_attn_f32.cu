@@ -216,8 +216,7 @@ static cudaError_t launch(const ptc_attn_args &a, Group group, int n_sm, cudaStr
     if (e != cudaSuccess) return e;
     if (per < 1) return cudaErrorInvalidConfiguration;
     const int grid = per * n_sm < FA_MAX_CTAS ? per * n_sm : FA_MAX_CTAS;
-    kernel<<<grid, FA_THREADS, smem, s>>>(a, group);
-    return cudaGetLastError();
+    return launch_kernel(kernel, grid, FA_THREADS, smem, s, a, group);
 }
 
 cudaError_t launch_attn_f32(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {

@@ -802,8 +802,7 @@ static cudaError_t launch_wide(const ptc_attn_args &a, Group group, int n_sm, cu
     const cudaError_t e = allow_smem(kernel, attn_smem(1024 + S::BYTES, ATTN_MAX_SEQS));
     if (e != cudaSuccess) return e;
     const long long fit = (long long)(PTC_ATTN_WORKSPACE_BYTES - ATTN_FLAG_BYTES) / (2 * S::SLOT * (int)sizeof(float));
-    kernel<<<(unsigned)(n_sm < fit ? n_sm : fit), WA_THREADS, smem, s>>>(a, wide_maps(a.cache), group);
-    return cudaGetLastError();
+    return launch_kernel(kernel, (unsigned)(n_sm < fit ? n_sm : fit), WA_THREADS, smem, s, a, wide_maps(a.cache), group);
 }
 
 cudaError_t launch_attn_wide(const ptc_attn_args &a, Group group, int n_sm, cudaStream_t s) {

@@ -226,8 +226,7 @@ extern "C" int ptc_plan_pages(const ptc_pages_args *p, void *stream) {
     if (smem > 48 * 1024)
         SERVE_CUDA(cudaFuncSetAttribute(ptc::k_plan_pages, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     const int want = (a.max_tokens + ptc::PLAN_THREADS - 1) / ptc::PLAN_THREADS;
-    ptc::k_plan_pages<<<want < 1 ? 1 : want < n_sm ? want : n_sm, ptc::PLAN_THREADS, smem, s>>>(a);
-    SERVE_CUDA(cudaGetLastError());
+    SERVE_CUDA(ptc::launch_kernel(ptc::k_plan_pages, want < 1 ? 1 : want < n_sm ? want : n_sm, ptc::PLAN_THREADS, smem, s, a));
     return 0;
 }
 
@@ -260,9 +259,9 @@ extern "C" int ptc_kv_append(const ptc_append_args *p, void *stream) {
     ptc::MemoryDevice on(a.q_out);
     SERVE_CUDA(on.error());
     const int cols = (int)(hd / u), lanes = ptc::AP_THREADS / cols;
-    if (a.cache.dtype == PTC_F32) ptc::k_kv_append<float><<<a.n_tokens, ptc::AP_THREADS, 0, s>>>(a, cols, lanes);
-    else if (a.cache.dtype == PTC_F16) ptc::k_kv_append<__half><<<a.n_tokens, ptc::AP_THREADS, 0, s>>>(a, cols, lanes);
-    else ptc::k_kv_append<__nv_bfloat16><<<a.n_tokens, ptc::AP_THREADS, 0, s>>>(a, cols, lanes);
-    SERVE_CUDA(cudaGetLastError());
+    const auto kernel = a.cache.dtype == PTC_F32   ? ptc::k_kv_append<float>
+                        : a.cache.dtype == PTC_F16 ? ptc::k_kv_append<__half>
+                                                   : ptc::k_kv_append<__nv_bfloat16>;
+    SERVE_CUDA(ptc::launch_kernel(kernel, a.n_tokens, ptc::AP_THREADS, 0, s, a, cols, lanes));
     return 0;
 }
