@@ -146,7 +146,7 @@ struct NarrowRows {
         }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const float ref = m[h] == -INFINITY ? 0.f : m[h];
+            const float ref = m[h] == -INFINITY ? 0.f : m[h] - Lift<T>::BY;
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll

@@ -205,6 +205,20 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
     return *(const uint32_t *)&v;
 }
 
+// Probabilities are 2^(score - reference + lift), for the product with V, the
+// sum and the outputs alike. f16 has no value between 0 and 2^-24, so that a
+// long tail of small ones would vanish from the product while it stands in the
+// sum; with a reference that is at most 2^8 too low (the kernels' rise), 2^7
+// more keep them below 2^15, inside its range, and the tail seven bits longer.
+template <typename T>
+struct Lift {
+    static constexpr float BY = 0.f;
+};
+template <>
+struct Lift<__half> {
+    static constexpr float BY = 7.f;
+};
+
 // 2^x by the special function unit (relative error 2^-22; 2^-inf is 0).
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;

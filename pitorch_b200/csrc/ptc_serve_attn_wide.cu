@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                                 tm_st16(o_tm + d, o);
                             }
                         }
-                        const float ref = m == -INFINITY ? 0.f : m;
+                        const float ref = m == -INFINITY ? 0.f : m - Lift<T>::BY;
                         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
