@@ -94,24 +94,28 @@ __device__ __forceinline__ double widen(float x) {
 struct Weigh {
     float top, most;    // the maximum, and the distance from it at which weights become zero
     float scale;        // bins per unit of distance
-    double c, topc;     // log2(e) / temperature, and times the maximum
+    double c, at;       // 256 log2(e) / temperature, and the maximum
     const double *table;
 
     // (the distance of an infinite maximum from itself is NaN: heavy, in bin 0)
     __device__ bool heavy(float x) const { return !(top - x >= most); }
     __device__ int bin(float x) const { return min(SP_BINS - 1, (int)((top - x) * scale)); }
-    // 2^y for y = (x - top) log2(e) / temperature: y = n/256 + r, 2^(n/256)
-    // from the table and the exponent, 2^r by its series (ln 2)^i / i!, to 2^-42
+    // 2^(y/256) for y = (x - top) c, n + r with |r| <= 1/2: 2^(n/256) from the
+    // table and the exponent, 2^(r/256) by its series (ln 2 / 256)^i / i!, to
+    // 2^-42. The difference comes first: it has an error of 2^-53 of itself, and
+    // none for logits of like size, wherever they are; a product with a logit of
+    // 10^5, or for a temperature of 0.01, would have one of the product.
     __device__ u64 weight(float x) const {
         if (!heavy(x)) return 0;
         if (x == top) return 1ull << 43;
         const double magic = 6755399441055744.0;   // 1.5 * 2^52: the sum's low bits are the rounded integer
-        const double y = fma(widen(x), c, -topc), t = fma(y, 256.0, magic);
+        const double diff = widen(x) - at, t = fma(diff, c, magic);
         const int n = __double2loint(t);
-        const double r = fma(t - magic, -1.0 / 256.0, y);
-        double p = 5.550410866482158e-2;
-        p = fma(p, r, 2.402265069591007e-1);
-        p = fma(p, r, 6.931471805599453e-1);
+        const double r = fma(diff, c, magic - t);
+        constexpr double ln = 0.6931471805599453 / 256.0;
+        double p = ln * ln * ln / 6.0;
+        p = fma(p, r, ln * ln / 2.0);
+        p = fma(p, r, ln);
         p = fma(p, r, 1.0) * table[n & 255];
         p = __hiloint2double(__double2hiint(p) + (((n >> 8) + 43) << 20), __double2loint(p));
         return (u64)__double_as_longlong(p + 4503599627370496.0) & ((1ull << 52) - 1);
@@ -482,10 +486,10 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
         if (tid == 0 && rank == 0) a.tokens[row] = at;
         return;
     }
-    const double c = 1.4426950408889634 / (double)temp;
+    const double c = 1.4426950408889634 / (double)temp;   // a logit's distance in powers of two
     // bins down to the lowest logit or to where weights end, whichever is nearer
     const float reach = fmaxf((float)(SP_RANGE / c), 1e-37f), spread = fminf(top - lowest, reach);
-    const Weigh wt = {top, reach, spread > 0.f ? fminf((SP_BINS - 1) / spread, 1e30f) : 1e30f, c, (double)top * c, sh.table};
+    const Weigh wt = {top, reach, spread > 0.f ? fminf((SP_BINS - 1) / spread, 1e30f) : 1e30f, 256.0 * c, (double)top, sh.table};
     R.wt = wt;
     const double least_w = ceil((mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE);
     const u64 least = least_w > 0 ? (u64)least_w : 0;   // min_p as a weight
