@@ -204,8 +204,9 @@ int ptc_paged_attention(const ptc_attn_args *a, void *stream);
  * which is never chosen; a row without any other logit gives -1. +inf logits
  * share the whole mass. The arrays are per row; temperature NULL means 1,
  * top_k, top_p or min_p NULL none of that rule. Weights are summed as 64-bit
- * integers (units of 2^-43 of the largest), so the token does not depend on
- * the order of any sum: the same inputs give the same tokens. */
+ * integers (units of 2^-43 of the largest; what is below half of one is never
+ * chosen), so the token does not depend on the order of any sum: the same
+ * inputs give the same tokens. */
 typedef struct {
     int dtype;              /* of the logits */
     int rows;

@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) k_sample(ptc_sample_args a, int
     }
     const double c = 1.4426950408889634 / (double)temp;   // a logit's distance in powers of two
     // bins down to the lowest logit or to where weights end, whichever is nearer
-    const float reach = fmaxf((float)(SP_RANGE / c), 1e-37f), spread = fminf(top - lowest, reach);
+    // (above 0 for every temperature)
+    const float reach = (float)(SP_RANGE / c), spread = fminf(top - lowest, reach);
     const Weigh wt = {top, reach, spread > 0.f ? fminf((SP_BINS - 1) / spread, 1e30f) : 1e30f, 256.0 * c, (double)top, sh.table};
     R.wt = wt;
     const double least_w = ceil((mp < 1.0f ? (double)mp : mp >= 1.0f ? 1.0 : 0.0) * SP_ONE);

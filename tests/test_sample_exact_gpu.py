@@ -49,3 +49,20 @@ def test_an_offset_of_all_logits_changes_nothing(ptlib):
         y = x + off
         assert torch.equal(y.double() - off, x.double())
         assert run_sample(ptlib, y, t, None, [0.95] * 64, None, u) == want
+
+
+def test_temperatures_at_the_low_end_of_the_type(ptlib):
+    """Weights are whole units of 2^-43 of the largest, so that what is below half of one is never chosen, not for u = 0
+    either, however small the distance and the temperature are."""
+    rows = [(t, d) for t in (1e-38, 3e-39, 1e-40, 1e-42, 3e-44, 1.5e-45) for d in (1.5e-37, 9.9e-38, 7e-38, 5e-38, 3.3e-38, 2.1e-38, 1.3e-38)]
+    x = torch.zeros(len(rows), 40, device="cuda")
+    t = torch.tensor([r[0] for r in rows])
+    x[:, :39] = -torch.tensor([r[1] for r in rows], device="cuda")[:, None]
+    assert bool((t > 0).all()) and bool((x[:, :39] < 0).all())
+    units = (x.double() / t.double().cuda()[:, None]).exp() * 2.0 ** 43
+    heavy = torch.where(units < 0.5, -math.inf, x)   # what has weight
+    for u in (0.0, 0.3, 0.9):
+        f = float(torch.tensor(u))
+        for p in (1.0, 0.9):
+            got = run_sample(ptlib, x, t.tolist(), None, [p] * len(rows), None, [u] * len(rows))
+            assert got == [sample_ref(heavy[i], float(t[i]), top_p=float(torch.tensor(p)), u=f) for i in range(len(rows))]
