@@ -111,7 +111,10 @@ int pt_prefill(pt_context_t *ctx, const int *tokens, int n);
 /* pt_forward_step with the next token sampled on the GPU: temperature (0:
  * greedy), top_k (0: off), top_p (1: off), min_p (0: off) from the caller's
  * uniform random number u in [0, 1); the rules are ptc_sample_tokens'. The
- * logits stay on the device unless ctx->sync_logits is set. */
+ * logits stay on the device when ctx->sync_logits is 0 (its default copies
+ * them as every step does). -1: a vocabulary above PTC_SAMPLE_MAX_VOCAB
+ * (ptc_serve.h; a message, ctx unchanged), or a step whose logits hold no
+ * number (the step is done, ctx->pos has moved on). */
 int pt_forward_step_sampled(pt_context_t *ctx, int token, float temperature,
                             int top_k, float top_p, float min_p, float u);
 

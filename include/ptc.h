@@ -163,7 +163,8 @@ void ptc_decoder_generate(ptc_decoder *d, const int *prompt, int n_prompt, int n
 int ptc_decoder_prefill(ptc_decoder *d, const int *tokens, int n, int pos0, float *logits_host);
 /* One token sampled on the device from the last step's logits, by the rules
  * of ptc_sample_tokens (ptc_serve.h; u uniform in [0, 1)). -1: no classifier,
- * no logit is a number, or (with a message) the last step's classifier was
+ * a vocabulary above PTC_SAMPLE_MAX_VOCAB, no logit is a number, or (with a
+ * message) the last step's classifier was
  * vocab-parallel and the other ranks' logits were not gathered: on the head
  * rank, pt_dist_forward_step gathers them while ctx->sync_logits is set, and
  * ptc_decoder_enqueue_fetch with logits says that its caller has. */

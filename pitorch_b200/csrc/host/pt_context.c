@@ -12,6 +12,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "../../../include/ptc_serve.h"
 #include "pt_device.h"
 
 void pt_fatal(const char *fmt, ...) {
@@ -266,6 +267,11 @@ int pt_prefill(pt_context_t *ctx, const int *tokens, int n) {
 
 int pt_forward_step_sampled(pt_context_t *ctx, int token, float temperature, int top_k, float top_p,
                             float min_p, float u) {
+    if (ctx->cfg.vocab_size > PTC_SAMPLE_MAX_VOCAB) {   /* before the step moves the context on */
+        fprintf(stderr, "pitorch_b200: pt_forward_step_sampled: vocabulary %d of at most %d\n", ctx->cfg.vocab_size,
+                PTC_SAMPLE_MAX_VOCAB);
+        return -1;
+    }
     int next = pt_forward_step(ctx, token);
     return next < 0 ? next : ptc_decoder_sample(ctx->dev->dec, temperature, top_k, top_p, min_p, u);
 }
