@@ -241,60 +241,58 @@ __device__ __forceinline__ void cp_async_wait() {
 // and 4 a thread or 4 outputs, whichever is more.
 template <typename T, int HDP, int MT, int SLOT, int THREADS>
 __device__ void attn_merge(const ptc_attn_args &a, const AttnItem &it, Group group, float *slots, int c0, int c1, float *smem) {
-                    // weights of the parts, a warp per row and a lane per part; then the
-                    // weighted sum, the parts shared out where there are few rows
-                    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = it.i1 - it.i0, hd = a.cache.head_dim, parts = c1 - c0 + 1;
-                    float *wgt = smem, *red = smem + (MT * parts + 3) / 4 * 4;
-                    auto part = [&](int p) { return slots + (long long)(2 * (c0 + p) + (p == 0)) * SLOT; };
-                    for (int r = warp; r < rows; r += THREADS / 32) {
-                        float top = -INFINITY, sum = 0.f;
-                        for (int p = lane; p < parts; p += 32) top = fmaxf(top, __ldcg(part(p) + MT * HDP + r));
-                        top = warp_max(top);
-                        const float ref = top == -INFINITY ? 0.f : top;
-                        for (int p = lane; p < parts; p += 32) {
-                            const float f = exp2f(__ldcg(part(p) + MT * HDP + r) - ref);
-                            wgt[r * parts + p] = f;
-                            sum += f * __ldcg(part(p) + MT * HDP + MT + r);
-                        }
-                        sum = warp_sum(sum);
-                        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-                        for (int p = lane; p < parts; p += 32) wgt[r * parts + p] *= inv;
-                    }
-                    __syncthreads();
-                    const int cols = rows * (HDP / 4), shares = max(1, THREADS / cols);
-                    for (int i = tid; i < cols * shares; i += THREADS) {
-                        const int share = i / cols, x = i % cols, r = x / (HDP / 4), d = x % (HDP / 4) * 4;
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    #pragma unroll 4
-                        for (int p = share; p < parts; p += shares) {
-                            const float f = wgt[r * parts + p];
-                            const float4 v = __ldcg((const float4 *)(part(p) + r * HDP + d));
-                            acc.x += f * v.x;
-                            acc.y += f * v.y;
-                            acc.z += f * v.z;
-                            acc.w += f * v.w;
-                        }
-                        *(float4 *)(red + i * 4) = acc;
-                    }
-                    __syncthreads();
-                    for (int x = tid; x < cols; x += THREADS) {
-                        const int r = x / (HDP / 4), d = x % (HDP / 4) * 4;
-                        if (d >= hd) continue;
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                        for (int share = 0; share < shares; share++) {
-                            const float4 v = *(const float4 *)(red + (share * cols + x) * 4);
-                            acc.x += v.x;
-                            acc.y += v.y;
-                            acc.z += v.z;
-                            acc.w += v.w;
-                        }
-                        const int row = it.i0 + r, tok = group.div(row);
-                        T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group.n + row - tok * group.n) * hd + d;
-                        dst[0] = Elem<T>::down(acc.x);
-                        dst[1] = Elem<T>::down(acc.y);
-                        dst[2] = Elem<T>::down(acc.z);
-                        dst[3] = Elem<T>::down(acc.w);
-                    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = it.i1 - it.i0, hd = a.cache.head_dim, parts = c1 - c0 + 1;
+    float *wgt = smem, *red = smem + (MT * parts + 3) / 4 * 4;
+    auto part = [&](int p) { return slots + (long long)(2 * (c0 + p) + (p == 0)) * SLOT; };
+    for (int r = warp; r < rows; r += THREADS / 32) {
+        float top = -INFINITY, sum = 0.f;
+        for (int p = lane; p < parts; p += 32) top = fmaxf(top, __ldcg(part(p) + MT * HDP + r));
+        top = warp_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        for (int p = lane; p < parts; p += 32) {
+            const float f = exp2f(__ldcg(part(p) + MT * HDP + r) - ref);
+            wgt[r * parts + p] = f;
+            sum += f * __ldcg(part(p) + MT * HDP + MT + r);
+        }
+        sum = warp_sum(sum);
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        for (int p = lane; p < parts; p += 32) wgt[r * parts + p] *= inv;
+    }
+    __syncthreads();
+    const int cols = rows * (HDP / 4), shares = max(1, THREADS / cols);
+    for (int i = tid; i < cols * shares; i += THREADS) {
+        const int share = i / cols, x = i % cols, r = x / (HDP / 4), d = x % (HDP / 4) * 4;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int p = share; p < parts; p += shares) {
+            const float f = wgt[r * parts + p];
+            const float4 v = __ldcg((const float4 *)(part(p) + r * HDP + d));
+            acc.x += f * v.x;
+            acc.y += f * v.y;
+            acc.z += f * v.z;
+            acc.w += f * v.w;
+        }
+        *(float4 *)(red + i * 4) = acc;
+    }
+    __syncthreads();
+    for (int x = tid; x < cols; x += THREADS) {
+        const int r = x / (HDP / 4), d = x % (HDP / 4) * 4;
+        if (d >= hd) continue;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int share = 0; share < shares; share++) {
+            const float4 v = *(const float4 *)(red + (share * cols + x) * 4);
+            acc.x += v.x;
+            acc.y += v.y;
+            acc.z += v.z;
+            acc.w += v.w;
+        }
+        const int row = it.i0 + r, tok = group.div(row);
+        T *dst = (T *)a.out + (it.s.q0 + tok) * a.out_stride + (long long)(it.head * group.n + row - tok * group.n) * hd + d;
+        dst[0] = Elem<T>::down(acc.x);
+        dst[1] = Elem<T>::down(acc.y);
+        dst[2] = Elem<T>::down(acc.z);
+        dst[3] = Elem<T>::down(acc.w);
+    }
 }
 
 // The kernel for many rows (ptc_serve_attn_wide.cu): 16-bit types, scale > 0.

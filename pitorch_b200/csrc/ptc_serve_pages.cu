@@ -223,8 +223,7 @@ extern "C" int ptc_plan_pages(const ptc_pages_args *p, void *stream) {
     int n_sm = 0;
     SERVE_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, on.device()));
     const size_t smem = (size_t)2 * (a.n_seqs + 1) * sizeof(int);
-    if (smem > 48 * 1024)
-        SERVE_CUDA(cudaFuncSetAttribute(ptc::k_plan_pages, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    static_assert(2 * (PTC_SERVE_MAX_SEQS + 1) * sizeof(int) <= 48 * 1024 - 512, "what a kernel has without asking");
     const int want = (a.max_tokens + ptc::PLAN_THREADS - 1) / ptc::PLAN_THREADS;
     SERVE_CUDA(ptc::launch_kernel(ptc::k_plan_pages, want < 1 ? 1 : want < n_sm ? want : n_sm, ptc::PLAN_THREADS, smem, s, a));
     return 0;
