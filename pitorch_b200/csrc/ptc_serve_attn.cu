@@ -516,13 +516,16 @@ extern "C" int ptc_paged_attention(const ptc_attn_args *p, void *stream) {
     SERVE_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, on.device()));
     const ptc::Group group(a.n_heads / a.cache.n_kv_heads);
     const long long most = (long long)(a.max_q < 1 ? 1 : a.max_q) * group.n;   // rows of a K/V head
-    // The kernel by the rows of the longest sequence. Measured at 8 K/V heads, few-rows kernel against many-rows kernel,
-    // us: 16-bit, 4 heads a group of 128, 16 sequences of about 1000 positions (64 of 250), 16 rows 42, 69 (48, 87); 32
-    // rows 78, 64 (82, 84); 64 rows 120, 65 (144, 90). f32, 1 head a group of 64, the same sequences: 12 rows 70, 100
-    // (78, 99); 16 rows 73, 100 (82, 95); 24 rows 108, 99 (123, 104).
+    // The kernel by the rows of the longest sequence: few rows are bound by reading the keys, which the few-rows kernel
+    // does with less to start, many by the products. Measured in a graph at 8 K/V heads, few-rows against many-rows
+    // kernel, us, for 16 sequences of about 1000 positions (64 of 250; 4 of 8000):
+    //   bf16, heads of 128  16 rows 29, 46 (37, 62; 46, 57)  32 rows 40, 46 (58, 61; 61, 58)  48 rows 52, 45 (79, 61; 77, 59)
+    //   f16, heads of 64    32 rows 27, 37 (37, 51; 39, 44)  48 rows 35, 38 (47, 50; 49, 44)  64 rows 42, 39 (58, 52; 54, 42)
+    //   f32, heads of 64    16 rows 46, 71 (65, 92)  24 rows 67, 84 (84, 93)  32 rows 92, 94 (114, 96)
+    //   f32, heads of 128   16 rows 96, 137 (137, 173)  24 rows 146, 154 (192, 177)  32 rows 207, 166 (260, 180)
     if (a.cache.dtype == PTC_F32) {
         // rows in registers: as many as the longest sequence fills, up to 8
-        if (most > 16) SERVE_CUDA(ptc::launch_attn_f32(a, group, n_sm, s));
+        if (most > 24) SERVE_CUDA(ptc::launch_attn_f32(a, group, n_sm, s));
         else if (most <= 1) SERVE_CUDA((ptc::launch_narrow_hd<float, 1>(a, group, n_sm, s)));
         else if (most <= 4) SERVE_CUDA((ptc::launch_narrow_hd<float, 4>(a, group, n_sm, s)));
         else SERVE_CUDA((ptc::launch_narrow_hd<float, 8>(a, group, n_sm, s)));
