@@ -105,7 +105,9 @@ void pt_generate_greedy(pt_context_t *ctx, const int *prompt, int n_prompt,
  * the greedy token after the last one (state.logits are that position's, as
  * after pt_forward_step), or -1 with ctx unchanged when the prompt does not
  * fit seq_len, a token is outside the vocabulary, or the context is a shard
- * (see ptc_decoder_prefill). */
+ * (see ptc_decoder_prefill). Its time hardly depends on n up to 256 tokens: steps
+ * are faster for the shortest prompts (below 13 tokens of the 15M model, 25 of
+ * the 110M model). */
 int pt_prefill(pt_context_t *ctx, const int *tokens, int n);
 
 /* pt_forward_step with the next token sampled on the GPU: temperature (0:

@@ -159,15 +159,16 @@ void ptc_decoder_generate(ptc_decoder *d, const int *prompt, int n_prompt, int n
  * as a step of that token would; -1 (with a message) for a decoder without
  * embedding, layers or head or with pipeline links, a head size that is no
  * multiple of 8, tokens outside the vocabulary or more than the positions that
- * are left. The first call takes buffers from the context's arena. */
+ * are left. The first call takes buffers from the context's arena: those of
+ * 256 rows and PTC_ATTN_WORKSPACE_BYTES. */
 int ptc_decoder_prefill(ptc_decoder *d, const int *tokens, int n, int pos0, float *logits_host);
 /* One token sampled on the device from the last step's logits, by the rules
  * of ptc_sample_tokens (ptc_serve.h; u uniform in [0, 1)). -1: no classifier,
  * a vocabulary above PTC_SAMPLE_MAX_VOCAB, no logit is a number, or (with a
- * message) the last step's classifier was
- * vocab-parallel and the other ranks' logits were not gathered: on the head
- * rank, pt_dist_forward_step gathers them while ctx->sync_logits is set, and
- * ptc_decoder_enqueue_fetch with logits says that its caller has. */
+ * message) the last step's classifier was vocab-parallel and the other ranks'
+ * logits were not gathered: on the head rank, pt_dist_forward_step gathers
+ * them while ctx->sync_logits is set, and ptc_decoder_enqueue_fetch with
+ * logits says that its caller has. */
 int ptc_decoder_sample(ptc_decoder *d, float temperature, int top_k, float top_p, float min_p, float u);
 
 /* Benchmark hooks: enqueue the device-loop step graph n times without

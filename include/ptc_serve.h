@@ -19,7 +19,8 @@
  * and returns -1; otherwise 0. What only the device can see -- lengths,
  * positions, page numbers -- is checked by the kernels: they OR a
  * PTC_SERVE_ERR_* bit into the device int *err (err may be NULL; the caller
- * clears it) and skip the access.
+ * clears it) and skip the access. Host threads may call at the same time, on
+ * streams of their own; a refused call does not show in a later one.
  */
 #ifndef PTC_SERVE_H
 #define PTC_SERVE_H
@@ -31,7 +32,8 @@ extern "C" {
 #endif
 
 /* Element types. Sums, softmax statistics and rotations are computed in 32
- * bits or more and rounded once to the type. */
+ * bits or more and rounded once to the type. What is rounded before that: the
+ * probabilities of 16-bit attention (see there). */
 enum { PTC_F32 = 0, PTC_F16 = 1, PTC_BF16 = 2 };
 
 enum {
@@ -50,7 +52,8 @@ enum {
 /* One step of n_seqs sequences, of which sequence r holds past_len[r] tokens
  * in the first ceil(past_len[r] / page_size) pages of its page_table row and
  * gets new_len[r] more (zero is fine for either). The pages it lacks are taken
- * from free_pages in order, sequence by sequence. Writes
+ * from free_pages in order, sequence by sequence; a page that stands there
+ * twice, or in the table too, is handed out all the same. Writes
  *   page_table[r][...]  the pages taken (entries that hold cached tokens and
  *                       entries behind the new ones are left as they are)
  *   kv_len[r]           past_len[r] + new_len[r]
@@ -153,7 +156,12 @@ int ptc_rope_table(float *table, int n_pos, int head_dim, void *stream);
  * A row that sees no position (p < 0) becomes zeros. One token per sequence,
  * chunks and mixtures of both are all one call; sequences may have no rows.
  * max_q is the largest number of rows of a sequence as far as the caller
- * knows it: it selects the kernel, not the result. Rows of q and out beyond
+ * knows it: it selects the kernel, whatever the rows are. The kernels agree
+ * up to their roundings: the one for few rows (16-bit types: up to 32 of a
+ * K/V head, heads of its group times max_q, or a scale of 0 or less) takes
+ * probabilities in two parts of the type, that for many rounds them to the type
+ * for the product with v, not for their sum. f16 probabilities are held in
+ * steps of 2^-31 of the largest weight or finer. Rows of q and out beyond
  * q_start[n_seqs] are neither read nor written. q_start has to rise from 0 to
  * at most n_tokens (LENGTH, the sequence is left out), kv_len may not pass
  * max_pages * page_size or 2^30 (LENGTH, positions behind it are left out), and

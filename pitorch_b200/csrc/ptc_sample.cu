@@ -28,7 +28,8 @@
 // Weights are integers in units of 2^-43 of the largest, so every sum is
 // exact, the order of the atomics has no effect, and the same row gives the
 // same token in any batch. They are computed in 64-bit arithmetic (2^y by a
-// table of 256 and a polynomial of degree 3, relative error below 2^-42): the
+// table of 256 and a polynomial of degree 3, relative error below 2^-42 wherever
+// the logits lie): the
 // running sum of 10^5 weights has to be exact to far better than the weight
 // of one token, which 32-bit exponentials do not give.
 //

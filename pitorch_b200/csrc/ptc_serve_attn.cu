@@ -17,9 +17,10 @@ namespace ptc {
 // take, so the unused rows cost little), f32 through fused multiply-adds on MT rows. Rows of a
 // stage are padded by 16 bytes, which keeps ldmatrix and the 128-bit reads
 // free of bank conflicts for every head size. Measured: 64 sequences of up to
-// 8192 positions, 32 heads in groups of 4, 128 elements of bf16: 209 us for
-// 1.08 GB of keys and values, 5.2 TB/s (0.79 of a measured copy; 0.84 without
-// the second product of the probabilities). One f32 token over 1024 positions
+// 8192 positions, 32 heads in groups of 4, 128 elements of bf16: 197 to 209 us for
+// 1.08 GB of keys and values, 5.2 to 5.5 TB/s (0.79 to 0.83 of a measured copy;
+// the second product of the probabilities takes 5% of it).
+// 64 f32 tokens over up to 1024 positions of 12 heads of 64: 64 us for 211 MB. One f32 token over 1024 positions
 // of 12 heads of 64: 8.9 us, of which the reads are 1: two searches of the work
 // table, the page lookup, one read, a counter and the sum of 16 parts follow
 // one another.

@@ -20,7 +20,8 @@
 //                   16-byte asynchronous copies where a run ends behind the last
 //                   position, and where page sizes are no multiple of 8
 // Measured: 4096 tokens behind 12288 cached ones, 32 heads in groups of 4, 128
-// elements of bf16: 0.96 ms, 1005 TFLOP/s (0.61 of the measured bf16 product);
+// elements of bf16: 0.96 to 1.05 ms from box to box and run to run, 1005 to 914
+// TFLOP/s (0.61 to 0.55 of the measured bf16 product);
 // the products alone take 0.72 ms and the softmax alone 0.68 ms. Exponentials
 // as polynomials on the multiply-add units were slower (1.03 ms with an eighth
 // of them, 1.06 with a quarter), and so were two copies of the softmax loop,
@@ -612,7 +613,10 @@ __global__ void __launch_bounds__(WA_THREADS, 1) k_attn_wide(ptc_attn_args a, co
                         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int q = 0; q < 2; q++) {
-                            // rounded to the type for the product with V (their sum is not)
+                            // rounded to the type for the product with V (their sum is not). What the rounding
+                            // leaves is not multiplied too, as the few-rows kernel does: that product would add half
+                            // of the products' time, and the output's own rounding is of the same size (error
+                            // of the long chunk against 64 bits 0.0023, of the output's rounding alone 0.0017).
                             uint32_t p[16];
 #pragma unroll
                             for (int k = 0; k < 32; k += 4) {
